@@ -396,6 +396,73 @@ int lampa_add_rmsnorm(float* res, const void* delta, int32_t delta_dtype, const 
                       const float* weight, float eps, int32_t delta_at_r, int32_t y_at_r, void* y,
                       int32_t y_dtype, int32_t* status, void* stream);
 /*
+ * Selective state space scan (a state of P x N per head, scalar decay per head and token) and its step.
+ *   d_t = softplus(dt_t + dt_bias[h]) (dt_softplus != 0), or dt_t + dt_bias[h];
+ *   h_t = exp(A[h] d_t) h_{t-1} + d_t x_t B_t^T;      y_t = (h_t C_t + D[h] x_t) * silu(z_t)
+ * Heads h of a group g = h / (H / G) share B and C.
+ */
+typedef struct lampa_ssm_desc {
+    int32_t B;           /* batch rows (1 when packed)                                       */
+    int32_t T;           /* tokens per batch row (all of them when packed)                   */
+    int32_t H;           /* heads                                                            */
+    int32_t P;           /* values per head                                                  */
+    int32_t N;           /* state size, at most 256                                          */
+    int32_t G;           /* groups of heads that share B and C; divides H                    */
+    int32_t nseq;        /* packed input: number of sequences (len(cu_seqlens) - 1), else 0  */
+    int32_t dtype;       /* of x, B, C, z and y: LAMPA_BF16 or LAMPA_F16 (step: any)         */
+    int32_t dt_dtype;    /* of dt                                                            */
+    int32_t dt_softplus;
+} lampa_ssm_desc;
+/* Scratch of lampa_ssm_scan, 16-byte aligned (0: none needed). */
+int lampa_ssm_workspace_bytes(const lampa_ssm_desc* d, size_t* bytes);
+/*
+ * x, z [B*T][H][P], B, C [B*T][G][N], dt [B*T][H]: the innermost axis is contiguous, the distances of the others are given in
+ * elements (*_tok from one token to the next, *_head / *_grp from one head / group to the next; heads of dt are neighbours), so that
+ * parts of a projection's rows are read in place.  y [B*T][H][P] dense.  A, D, dt_bias [H] fp32 (D, dt_bias, z may be NULL).
+ * initial_state, final_state [N_seq][H][P][N] fp32 or NULL, N_seq = nseq or B; they may be the same array.
+ * cu_seqlens: device int64 [nseq+1] rising from 0; rows of y behind its last entry are zero; an entry that falls or leaves the
+ * input sets LAMPA_ERR_BOUNDS and leaves that sequence's outputs undefined.  Every state is found and kept in fp32 (relative
+ * error below 1e-6); y has one rounding to the input type on the way and its own.  An x, dt, B, C that is not finite spoils its
+ * sequence from its token on (a C: its token) and nothing else.
+ */
+int lampa_ssm_scan(const lampa_ssm_desc* d, const void* x, int64_t x_tok, int64_t x_head, const void* dt, int64_t dt_tok,
+                   const float* A, const void* B, int64_t b_tok, int64_t b_grp, const void* C, int64_t c_tok, int64_t c_grp,
+                   const float* D, const void* z, int64_t z_tok, int64_t z_head, const float* dt_bias, const float* initial_state,
+                   const int64_t* cu_seqlens, void* y, float* final_state, void* ws, size_t ws_bytes, int32_t* status, void* stream);
+/*
+ * One token per batch row through the short convolution in front of the recurrence and the recurrence itself, in one launch:
+ * xbc [B] rows of H*P + 2*G*N channels (x, then B, then C), xbc_row elements apart; conv_cache [B][channels][taps] (dtype, the
+ * layout of lampa_short_conv_step) moves one slot left and takes xbc; conv_weight [channels][taps] and conv_bias [channels] (or
+ * NULL) of w_dtype, taps 2 to 8; silu: activation behind the convolution.  state [B][H][P][N] fp32, in place.  dt [B] rows of H.
+ * y [B][H][P].  The convolution's result is used in fp32, without a rounding to `dtype`.
+ */
+int lampa_ssm_step(const lampa_ssm_desc* d, const void* xbc, int64_t xbc_row, const void* dt, int64_t dt_row, void* conv_cache,
+                   const void* conv_weight, const void* conv_bias, int32_t taps, int32_t w_dtype, int32_t silu, const float* A,
+                   const float* D, const void* z, int64_t z_row, int64_t z_head, const float* dt_bias, float* state, void* y,
+                   void* stream);
+/*
+ * Short convolution of a prompt that continues: as lampa_short_conv_fwd, but what lies before a sequence's first token is what
+ * cache [nseq][D][W] holds (NULL: zero), and with write_cache the cache becomes the last W inputs of the sequence, earlier ones
+ * included (in place; that of an empty sequence stays).  x [n_tok] rows of D elements, x_row apart; y [n_tok][D] dense; without
+ * cu_seqlens n_tok / nseq tokens per sequence.  Rows of y behind the last entry of cu_seqlens are zero.  W 2 to 8.
+ */
+int lampa_short_conv_resume(const void* x, int64_t x_row, const void* weight, const void* bias, const int64_t* cu_seqlens,
+                            int32_t nseq, int64_t n_tok, int32_t D, int32_t W, int32_t dtype, int32_t w_dtype, int32_t silu,
+                            void* cache, int32_t write_cache, void* y, int32_t* status, void* stream);
+/*
+ * Norms before and after a block on its fp32 residual stream res [rows][D], in place:
+ *   n = delta / sqrt(mean(delta^2) + eps) * post_weight     (post_norm == 0: n = delta * post_weight)
+ *   res += scale * act(gate) * n                             (scale [D], or scale_all when scale is NULL)
+ *   y = res / sqrt(mean(res^2) + eps) * pre_weight           (y NULL: the update only; delta NULL: this norm only)
+ * delta [rows] rows delta_row apart; gate: one row per row, or with cu_seqlens one per sequence, gate_row apart (0: the same for
+ * all); gate_act 0 none, 1 sigmoid, 2 silu; weights [D] fp32 or NULL.  With cu_seqlens a row of no sequence has no gate: its res
+ * stays.  D at most 8192.
+ */
+int lampa_block_norm(float* res, const void* delta, int64_t delta_row, int32_t delta_dtype, const void* gate, int64_t gate_row,
+                     int32_t gate_dtype, int32_t gate_act, const int64_t* cu_seqlens, int32_t nseq, int64_t rows, int32_t D,
+                     const float* post_weight, int32_t post_norm, const float* scale, float scale_all, const float* pre_weight,
+                     float eps, void* y, int32_t y_dtype, int32_t* status, void* stream);
+/*
  * Bucketed RBF-kernel attention of the HEPT layer, fp32.  Per (round, head) the n hits are taken in
  * the order q_pos / k_pos (int64 [rounds][heads][n]; NULL: rows are already in order), cut into
  * buckets of `bucket` consecutive hits (n % bucket == 0, bucket <= 128), and inside a bucket

@@ -34,6 +34,10 @@ class GdnDesc(ctypes.Structure):
                 ("use_l2norm", ctypes.c_int32), ("scale", ctypes.c_float)]
 
 
+class SsmDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("B", "T", "H", "P", "N", "G", "nseq", "dtype", "dt_dtype", "dt_softplus")]
+
+
 _lib: Optional[ctypes.CDLL] = None
 EXPORTS = ["lampa_version", "lampa_error_string", "lampa_gdn_workspace_bytes", "lampa_gdn_workspace_layout",
            "lampa_gdn_fwd", "lampa_hgdn_fwd", "lampa_hgdn_fwd_scatter", "lampa_hgdn_final_state", "lampa_hgdn_prefill",
@@ -44,6 +48,7 @@ EXPORTS = ["lampa_version", "lampa_error_string", "lampa_gdn_workspace_bytes", "
            "lampa_row_range", "lampa_quantile_regions", "lampa_geo_keys",
            "lampa_hept_front_blocks", "lampa_hept_front", "lampa_geo_keys_fused", "lampa_region_inputs",
            "lampa_bucket_rbf_attn", "lampa_bucket_rbf_attn_checked", "lampa_bucket_attn_combine", "lampa_hept_prep_qk",
+           "lampa_ssm_workspace_bytes", "lampa_ssm_scan", "lampa_ssm_step", "lampa_short_conv_resume", "lampa_block_norm",
            "lampa_hgdn_fwd_again", "lampa_model_encode", "lampa_model_project", "lampa_model_update", "lampa_model_head",
            "lampa_repeat_segments", "lampa_profile_enable",
            "lampa_profile_read", "lampa_debug_set_poll_budget", "lampa_debug_set_tick_buffer",
@@ -93,6 +98,13 @@ def lib() -> ctypes.CDLL:
         L.lampa_gate_inputs.argtypes = [vp] * 7 + [i64, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp]
         L.lampa_rmsnorm_gate.argtypes = [vp, vp, vp, i64, i32, i32, i32, ctypes.c_float, i32, vp, vp]
         L.lampa_add_rmsnorm.argtypes = [vp, vp, i32, vp, vp, i32, i64, i32, vp, ctypes.c_float, i32, i32, vp, i32, vp, vp]
+        sd, f32 = ctypes.POINTER(SsmDesc), ctypes.c_float
+        L.lampa_ssm_workspace_bytes.argtypes = [sd, ctypes.POINTER(sz)]
+        L.lampa_ssm_scan.argtypes = [sd, vp, i64, i64, vp, i64, vp, vp, i64, i64, vp, i64, i64, vp, vp, i64, i64, vp, vp, vp, vp, vp, vp, sz,
+                                     vp, vp]
+        L.lampa_ssm_step.argtypes = [sd, vp, i64, vp, i64, vp, vp, vp, i32, i32, i32, vp, vp, vp, i64, i64, vp, vp, vp, vp]
+        L.lampa_short_conv_resume.argtypes = [vp, i64, vp, vp, vp, i32, i64, i32, i32, i32, i32, i32, vp, i32, vp, vp, vp]
+        L.lampa_block_norm.argtypes = [vp, vp, i64, i32, vp, i64, i32, i32, vp, i32, i64, i32, vp, i32, vp, f32, vp, f32, vp, i32, vp, vp]
         L.lampa_repeat_segments.argtypes = [vp, i32, i32, i64, vp, vp]
         L.lampa_profile_enable.argtypes = [ctypes.c_int]
         L.lampa_debug_set_poll_budget.argtypes = [ctypes.c_int]

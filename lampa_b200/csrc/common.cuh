@@ -288,6 +288,14 @@ __device__ __forceinline__ int64_t highest_offset(int64_t t, int64_t total, int6
     return top;
 }
 
+// Whether packed offsets rise from 0 and stay inside the rows, reported by the threads of one CTA
+__device__ __forceinline__ void check_offsets(const int64_t* cu, int nseq, int64_t rows, int32_t* status, int where) {
+    for (int i = threadIdx.y * blockDim.x + threadIdx.x; i < nseq; i += blockDim.x * blockDim.y) {
+        const int64_t b = cu[i], e = cu[i + 1];
+        if (e < b || e > rows || (i == 0 && b != 0)) set_status(status, LAMPA_ERR_BOUNDS, where, i);
+    }
+}
+
 // index of the sequence whose [off[s], off[s+1]) contains x (off non-decreasing; empty ranges skipped)
 __device__ __forceinline__ int find_seq(const int32_t* off, int nseq, int x) {
     int lo = 0, hi = nseq;            // invariant: off[lo] <= x < off[hi]

@@ -11,6 +11,7 @@
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -290,6 +291,7 @@ PyObject* step(PyObject* const* a) {
 #include "host_lsh.inc"
 #include "host_model.inc"
 #include "host_hept.inc"
+#include "host_ssm.inc"
 
 template <PyObject* (*F)(PyObject* const*), int N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -309,6 +311,7 @@ PyMethodDef methods[] = {
     ENTRY(gdn, 13), ENTRY(prefill, 7), ENTRY(step, 10),
     ENTRY(lsh_hash, 8), ENTRY(segsort, 4), ENTRY(permute_rows, 5), ENTRY(invert_perm, 1), ENTRY(bucket_sort, 4), ENTRY(ordering, 3),
     ENTRY(model_forward, 6), ENTRY(region_inputs, 3), ENTRY(hept_core, 11),
+    ENTRY(ssm_scan, 13), ENTRY(ssm_step, 13), ENTRY(conv_resume, 8), ENTRY(block_norm, 12),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "Native host path of lampa_b200", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -9,48 +9,13 @@
 #include "act.cuh"
 #include "common.cuh"
 #include "profile.cuh"
+#include "vec.cuh"
 #include <algorithm>
 
 namespace lampa {
 
 constexpr int CONV_MAX_W = 8;       // taps
 constexpr int CONV_TOKENS = 16;     // consecutive tokens per thread (window kept in registers)
-
-template <int DT> struct Vec16;     // 16 bytes of channels
-template <> struct Vec16<LAMPA_F32> { static constexpr int N = 4; };
-template <> struct Vec16<LAMPA_BF16> { static constexpr int N = 8; };
-template <> struct Vec16<LAMPA_F16> { static constexpr int N = 8; };
-
-template <int DT>
-__device__ __forceinline__ void unpack_vec(const uint4& u, float (&x)[Vec16<DT>::N]) {
-    if (DT == LAMPA_F32) {
-        x[0] = __uint_as_float(u.x); x[1] = __uint_as_float(u.y); x[2] = __uint_as_float(u.z); x[3] = __uint_as_float(u.w);
-    } else {
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float2 f;
-            if (DT == LAMPA_BF16) f = unpack_bf16x2(w[j]);
-            else f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-            x[2 * j] = f.x; x[2 * j + 1] = f.y;
-        }
-    }
-}
-template <int DT>
-__device__ __forceinline__ void store_vec(void* p, size_t elem, const float (&x)[Vec16<DT>::N]) {
-    uint4 u;
-    if (DT == LAMPA_F32) {
-        u = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
-    } else if (DT == LAMPA_BF16) {
-        u = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
-    } else {
-        __half2 h[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
-        u = *reinterpret_cast<const uint4*>(h);
-    }
-    *reinterpret_cast<uint4*>((char*)p + elem * (DT == LAMPA_F32 ? 4 : 2)) = u;
-}
 
 // Four channels of one token: 8 bytes of bf16 / fp16, 16 bytes of fp32.
 template <int DT> struct Raw4 { using T = uint2; };

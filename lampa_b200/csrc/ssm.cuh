@@ -1,0 +1,76 @@
+// Selective state space scan: arguments and positions shared by its kernels.
+//   h_t = exp(A d_t) h_{t-1} + d_t x_t B_t^T  (P x N per head),   y_t = (h_t C_t + D x_t) silu(z_t),
+//   d_t = softplus(dt_t + dt_bias) or the sum itself.
+#pragma once
+#include "act.cuh"
+#include "common.cuh"
+
+namespace lampa {
+
+constexpr int SSM_Q = 64;             // tokens per chunk of the mma.sync kernels
+
+struct SsmArgs {
+    const void* x; const void* dt; const void* B; const void* C; const void* z;
+    const float* A; const float* D; const float* dt_bias; const float* h0;
+    const int64_t* cu;
+    void* y; float* ht;
+    float* blk;                       // [units][H][P][N]: end states of blocks that begin empty, then the states that enter them
+    float* blk_dec;                   // [units][H]: log decay of a block
+    int32_t* status;
+    int64_t x_tok, x_head, z_tok, z_head, b_tok, b_grp, c_tok, c_grp, dt_tok;   // distances in elements
+    int64_t n_tok, T;                 // rows in all; tokens per sequence without cu
+    int nseq;                         // sequences
+    int nb;                           // blocks per sequence without cu
+    int bl;                           // tokens per block
+    int H, P, N, G, dt_dt, softplus;
+    int vec;                          // rows of x, B and C are 16-byte aligned
+    int poll_budget;
+};
+
+// A block of tokens that one CTA walks through.  Packed sequences need no table: block b of sequence s has the number
+// floor(cu[s] / bl) + s + b, which rises strictly through all blocks of all sequences in order (some numbers stay unused), so
+// that a CTA finds its sequence by bisection.  What lies behind the last offset counts as one more sequence.
+struct SsmUnit {
+    int seq;
+    int64_t bos, eos, t0, t1;         // the sequence, and this block of it
+    bool outside;                     // behind the last sequence
+    __device__ __forceinline__ bool single(int bl) const { return eos - bos <= bl; }
+};
+__device__ __forceinline__ bool ssm_unit(const SsmArgs& a, int u, SsmUnit& r) {
+    int64_t b;
+    if (a.cu == nullptr) {
+        r.seq = u / a.nb;
+        b = u - r.seq * a.nb;
+        r.bos = (int64_t)r.seq * a.T;
+        r.eos = r.bos + a.T;
+        r.outside = false;
+    } else {
+        int lo = 0, hi = a.nseq + 1;  // largest s with floor(cu[s] / bl) + s <= u
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (a.cu[mid] / a.bl + mid <= u) lo = mid; else hi = mid;
+        }
+        r.seq = lo;
+        r.outside = lo == a.nseq;
+        r.bos = a.cu[lo];
+        r.eos = r.outside ? a.n_tok : a.cu[lo + 1];
+        if (r.bos < 0 || r.eos < r.bos || r.eos > a.n_tok) return false;      // reported by check_offsets
+        b = u - (r.bos / a.bl + lo);
+        if (b < 0) return false;
+    }
+    r.t0 = r.bos + b * a.bl;
+    r.t1 = min(r.eos, r.t0 + a.bl);
+    return r.t0 < r.eos;
+}
+inline int64_t ssm_units(int64_t n_tok, int nseq, int nb, int bl, bool packed) {
+    return packed ? n_tok / bl + nseq + 1 : (int64_t)nseq * nb;
+}
+
+// log(1 + e^x) to fp32 rounding: the states are kept to a few parts in 10^7, and softplusf_ is good to 2e-7 of 1
+__device__ __forceinline__ float ssm_step_size(float v, int softplus) {
+    return softplus ? fmaxf(v, 0.f) + log1pf(expf(-fabsf(v))) : v;
+}
+
+int launch_ssm_scan_mma(const SsmArgs& a, int dtype, int units, bool blocks, cudaStream_t st);
+
+}  // namespace lampa

@@ -1,0 +1,428 @@
+// Selective state space scan over whole sequences, mma.sync form: any head dims, bf16 and fp16.
+//
+// Inside a chunk of 64 tokens, with G_i the running sum of A d, the output is a masked matrix product,
+//   y_i = sum_{j <= i} (C_i . B_j) e^{G_i - G_j} d_j x_j + e^{G_i} S C_i,        S <- e^{G_last} S + sum_j e^{G_last - G_j} d_j x_j B_j^T,
+// so a CTA that walks through a block of chunks keeps one P x N state in registers (fp32) and reads every token once.  One sequence
+// has few heads, so its tokens are cut into blocks as well: a first kernel finds what each block makes of an empty state, a second
+// runs over the blocks, a third walks through the tokens again from the states that enter the blocks.
+//
+// Accuracy.  Operands of the tensor cores are bf16; fp16 inputs are taken as two bf16 pieces, exactly.  What a caller sees in 16
+// bits (y) has one rounding of the scores, or of the state, to the input's precision before its own.  States are seen in fp32: their
+// updates take d x e^{..} in three bf16 pieces (24 bits), and chunk sums are added in fp32 arithmetic.
+//
+// A token whose x is not finite must not reach the rows in front of it through a zero of the mask (0 * NaN): such elements are taken
+// out of the tile, and from their row on the column is NaN, as the recurrence has it.
+#include "profile.cuh"
+#include "ssm.cuh"
+
+#include <algorithm>
+
+namespace lampa {
+namespace {
+
+constexpr int Q = SSM_Q;
+constexpr int THREADS = 128;
+
+template <int DT> struct Raw16 { using T = __nv_bfloat16; };
+template <> struct Raw16<LAMPA_F16> { using T = __half; };
+
+__device__ __forceinline__ bool finite_(float v) { return fabsf(v) <= 3.402823466e38f; }
+
+template <int DT, int NP, int PT>
+struct Sm {
+    static constexpr int XP = DT == LAMPA_F16 ? 2 : 1;                 // bf16 pieces of an input
+    static constexpr int LN = NP + 8, LP = PT + 8;                     // row pitches: 16 bytes more than a power of two
+    __nv_bfloat16 B[XP][Q * LN];
+    __nv_bfloat16 C[XP][Q * LN];
+    __nv_bfloat16 S[XP][PT * LN];                                      // state as the right operand of C S^T
+    __nv_bfloat16 x[XP][Q * LP];
+    __nv_bfloat16 wx[3][Q * LP];                                       // d x e^{G_last - G}
+    float G[Q], d[Q], w[Q];
+    int bad[PT];                                                       // first row of the column that is not finite, or Q
+};
+
+// rows [0, n) of a matrix of 16-bit elements into [Q][ld] tiles of XP pieces, zero beyond n rows and `cols` columns.
+// FIND: elements that are not finite become zero and leave their row in bad[].
+template <int DT, int XP, int COLS, bool FIND>
+__device__ __forceinline__ void load_tile(__nv_bfloat16* dst, int piece, int ld, const void* base, int64_t off, int64_t pitch, int n, int cols,
+                                          bool vec, int* bad) {
+    using T = typename Raw16<DT>::T;
+    const T* src = (const T*)base + off;
+    for (int i = threadIdx.x; i < Q * (COLS / 8); i += THREADS) {
+        const int r = i / (COLS / 8), c = (i % (COLS / 8)) * 8;
+        uint4 u = make_uint4(0u, 0u, 0u, 0u);
+        if (r < n && c < cols) {
+            const T* p = src + (int64_t)r * pitch + c;
+            if (vec) u = __ldg(reinterpret_cast<const uint4*>(p));     // cols is a multiple of 8 then
+            else {
+                uint16_t e[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) e[k] = c + k < cols ? __ldg(reinterpret_cast<const uint16_t*>(p) + k) : (uint16_t)0;
+                u = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+            }
+        }
+        uint32_t w[4] = {u.x, u.y, u.z, u.w}, lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float2 f = DT == LAMPA_F16 ? __half22float2(*reinterpret_cast<__half2*>(&w[k])) : unpack_bf16x2(w[k]);
+            if (FIND) {
+                const bool f0 = finite_(f.x), f1 = finite_(f.y);
+                if (!f0) { atomicMin(&bad[c + 2 * k], r); f.x = 0.f; }
+                if (!f1) { atomicMin(&bad[c + 2 * k + 1], r); f.y = 0.f; }
+            }
+            w[k] = pack_bf16x2(f.x, f.y);
+            if (XP > 1) {
+                const float2 h = unpack_bf16x2(w[k]);
+                lo[k] = pack_bf16x2(f.x - h.x, f.y - h.y);
+            }
+        }
+        *reinterpret_cast<uint4*>(dst + r * ld + c) = make_uint4(w[0], w[1], w[2], w[3]);
+        if (XP > 1) *reinterpret_cast<uint4*>(dst + piece + r * ld + c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+}
+
+// d, G and w = d e^{G_last - G} of a chunk's n tokens (tokens beyond them have d = 0).  Returns G_last.  The first warp computes,
+// everybody else comes in behind the caller's barrier.  The exponent of w is summed from the end of the chunk: it then carries an
+// error of its own size, not of G's.
+template <typename SM>
+__device__ __forceinline__ void chunk_steps(const SsmArgs& a, SM& s, int64_t t0, int n, int h) {
+    if (threadIdx.x >= 32) return;
+    const int l = threadIdx.x;
+    const float A = a.A[h], bias = a.dt_bias ? a.dt_bias[h] : 0.f;
+    float d[2], g[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int i = 2 * l + k;
+        d[k] = i < n ? ssm_step_size(load_as_float(a.dt, (size_t)((t0 + i) * a.dt_tok + h), a.dt_dt) + bias, a.softplus) : 0.f;
+        g[k] = i < n ? d[k] * A : 0.f;
+    }
+    float up = g[0] + g[1], down = up;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const float u = __shfl_up_sync(0xffffffffu, up, o), v = __shfl_down_sync(0xffffffffu, down, o);
+        if (l >= o) up += u;
+        if (l + o < 32) down += v;
+    }
+    const float before = __shfl_up_sync(0xffffffffu, up, 1), after = __shfl_down_sync(0xffffffffu, down, 1);
+    const float b = l ? before : 0.f, e = l < 31 ? after : 0.f;
+    s.d[2 * l] = d[0]; s.d[2 * l + 1] = d[1];
+    s.G[2 * l] = b + g[0]; s.G[2 * l + 1] = up;
+    s.w[2 * l] = d[0] * expf(e + g[1]);
+    s.w[2 * l + 1] = d[1] * expf(e);
+}
+
+// wx pieces from the x tile: `pieces` of three
+template <int DT, int NP, int PT>
+__device__ __forceinline__ void scale_x(Sm<DT, NP, PT>& s, int pieces) {
+    using S = Sm<DT, NP, PT>;
+    for (int i = threadIdx.x; i < Q * (PT / 2); i += THREADS) {
+        const int r = i / (PT / 2), c = (i % (PT / 2)) * 2, at = r * S::LP + c;
+        float2 v = unpack_bf16x2(*reinterpret_cast<const uint32_t*>(&s.x[0][at]));
+        if (S::XP > 1) {
+            const float2 lo = unpack_bf16x2(*reinterpret_cast<const uint32_t*>(&s.x[S::XP - 1][at]));
+            v.x += lo.x; v.y += lo.y;
+        }
+        v.x *= s.w[r]; v.y *= s.w[r];
+        for (int p = 0; p < pieces; ++p) {
+            const uint32_t u = pack_bf16x2(v.x, v.y);
+            *reinterpret_cast<uint32_t*>(&s.wx[p][at]) = u;
+            const float2 h = unpack_bf16x2(u);
+            v.x -= h.x; v.y -= h.y;
+        }
+    }
+}
+
+// The state of a CTA: PT x NP, warp w holds rows 16 (w % RS) .. +15 and columns of 16 (cg + CG i)
+template <int NP, int PT>
+struct StateMap {
+    static constexpr int RS = PT / 16, CG = 4 / RS;
+    static constexpr int CT = NP / 16 >= CG ? NP / 16 / CG : 1;
+};
+
+// S <- dec S + sum_j wx_j B_j^T.  Every chunk sum starts from zero and is added in fp32 arithmetic (an MMA that accumulates onto a
+// long sum rounds it towards zero each time); smallest pieces first.
+template <int DT, int NP, int PT>
+__device__ __forceinline__ void update_state(float (&st)[StateMap<NP, PT>::CT][2][4], const Sm<DT, NP, PT>& s, float dec, int pieces) {
+    using M = StateMap<NP, PT>;
+    using S = Sm<DT, NP, PT>;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, p0 = 16 * (warp % M::RS), cg = warp / M::RS;
+#pragma unroll
+    for (int i = 0; i < M::CT; ++i) {
+        const int n0 = 16 * (cg + M::CG * i);
+        if (n0 >= NP) continue;
+        float c[2][4] = {};
+#pragma unroll 1
+        for (int p = pieces - 1; p >= 0; --p)
+#pragma unroll
+            for (int bp = S::XP - 1; bp >= 0; --bp)
+#pragma unroll
+                for (int k = 0; k < Q; k += 16) {
+                    uint32_t av[4], bv[4];
+                    load_a_t(av, s.wx[p], S::LP, p0, k, lane);
+                    load_b_t(bv, s.B[bp], S::LN, n0, k, lane);
+                    mma16816(c[0], av, bv[0], bv[1]);
+                    mma16816(c[1], av, bv[2], bv[3]);
+                }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) st[i][t][q] = fmaf(dec, st[i][t][q], c[t][q]);
+    }
+}
+
+// f(p, n, value) over the state elements of this thread
+template <int NP, int PT, typename F>
+__device__ __forceinline__ void each_state(float (&st)[StateMap<NP, PT>::CT][2][4], F f) {
+    using M = StateMap<NP, PT>;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, p0 = 16 * (warp % M::RS), cg = warp / M::RS;
+#pragma unroll
+    for (int i = 0; i < M::CT; ++i) {
+        const int n0 = 16 * (cg + M::CG * i);
+        if (n0 >= NP) continue;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) f(p0 + (lane >> 2) + 8 * (q >> 1), n0 + 8 * t + 2 * (lane & 3) + (q & 1), st[i][t][q]);
+    }
+}
+
+// What every block makes of an empty state.  A block that is its whole sequence needs no such state.
+template <int DT, int NP, int PT>
+__global__ void __launch_bounds__(THREADS) ssm_state_kernel(SsmArgs a) {
+    if (chain_wait()) return;
+    extern __shared__ __align__(16) char raw[];
+    Sm<DT, NP, PT>& s = *reinterpret_cast<Sm<DT, NP, PT>*>(raw);
+    SsmUnit u;
+    const int h = blockIdx.y, p0 = blockIdx.z * PT;
+    if (!ssm_unit(a, blockIdx.x, u) || u.outside || u.single(a.bl)) return;
+    float st[StateMap<NP, PT>::CT][2][4] = {};
+    float log_dec = 0.f;
+    for (int64_t t = u.t0; t < u.t1; t += Q) {
+        const int n = (int)min((int64_t)Q, u.t1 - t);
+        __syncthreads();
+        chunk_steps(a, s, t, n, h);
+        load_tile<DT, Sm<DT, NP, PT>::XP, NP, false>(s.B[0], Q * Sm<DT, NP, PT>::LN, Sm<DT, NP, PT>::LN, a.B, t * a.b_tok + (h / (a.H / a.G)) * a.b_grp, a.b_tok, n, a.N, a.vec, nullptr);
+        load_tile<DT, Sm<DT, NP, PT>::XP, PT, false>(s.x[0], Q * Sm<DT, NP, PT>::LP, Sm<DT, NP, PT>::LP, a.x, t * a.x_tok + h * a.x_head + p0, a.x_tok, n, a.P - p0, a.vec, nullptr);
+        __syncthreads();
+        scale_x(s, 3);
+        __syncthreads();
+        const float g = s.G[Q - 1];
+        update_state(st, s, expf(g), 3);
+        log_dec += g;
+    }
+    float* out = a.blk + ((int64_t)blockIdx.x * a.H + h) * a.P * a.N;
+    each_state<NP, PT>(st, [&](int p, int n, float v) {
+        if (p0 + p < a.P && n < a.N) out[(int64_t)(p0 + p) * a.N + n] = v;
+    });
+    if (threadIdx.x == 0 && blockIdx.z == 0) a.blk_dec[(int64_t)blockIdx.x * a.H + h] = log_dec;
+}
+
+// Over the blocks of a sequence: what enters each of them takes the place of what it makes of an empty state.  Also the final state,
+// but for sequences of one block, whose only CTA writes it.
+__global__ void __launch_bounds__(256) ssm_pass_kernel(SsmArgs a) {
+    if (chain_wait()) return;
+    const int pn = a.P * a.N, slabs = (pn + 255) / 256, seq = blockIdx.x / slabs, h = blockIdx.y;
+    const int e = (blockIdx.x - seq * slabs) * 256 + threadIdx.x;
+    int64_t bos = (int64_t)seq * a.T, eos = bos + a.T, u0 = (int64_t)seq * a.nb;
+    if (a.cu) {
+        bos = a.cu[seq]; eos = a.cu[seq + 1];
+        if (bos < 0 || eos < bos || eos > a.n_tok) return;         // reported by the output kernel
+        u0 = bos / a.bl + seq;
+    }
+    if (e >= pn) return;
+    const int64_t len = eos - bos, out = ((int64_t)seq * a.H + h) * pn + e;
+    float s = a.h0 ? a.h0[out] : 0.f;
+    if (len > a.bl) {
+        const int nb = (int)((len + a.bl - 1) / a.bl);
+        float* p = a.blk + (u0 * a.H + h) * pn + e;
+        const float* dec = a.blk_dec + u0 * a.H + h;
+        for (int b = 0; b < nb; ++b) {
+            const float part = *p;
+            *p = s;
+            s = fmaf(expf(*dec), s, part);
+            p += (int64_t)a.H * pn;
+            dec += a.H;
+        }
+    } else if (len > 0) return;
+    if (a.ht) a.ht[out] = s;
+}
+
+template <int DT>
+__device__ __forceinline__ float load16(const void* p, int64_t i) { return Elem<DT>::ld(p, (size_t)i); }
+
+template <int DT, int NP, int PT>
+__global__ void __launch_bounds__(THREADS) ssm_out_kernel(SsmArgs a) {
+    using SMT = Sm<DT, NP, PT>;
+    constexpr int XP = SMT::XP, LN = SMT::LN, LP = SMT::LP;
+    if (chain_wait()) return;
+    extern __shared__ __align__(16) char raw[];
+    SMT& s = *reinterpret_cast<SMT*>(raw);
+    SsmUnit u;
+    const int h = blockIdx.y, p0 = blockIdx.z * PT, grp = h / (a.H / a.G);
+    if (a.cu && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) check_offsets(a.cu, a.nseq, a.n_tok, a.status, 50);
+    if (!ssm_unit(a, blockIdx.x, u)) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t2 = 2 * (lane & 3);
+    if (u.outside) {                                               // rows of no sequence read as zero
+        for (int64_t i = threadIdx.x; i < (u.t1 - u.t0) * PT; i += THREADS) {
+            const int p = p0 + (int)(i % PT);
+            if (p < a.P) Elem<DT>::st(a.y, (size_t)(((u.t0 + i / PT) * a.H + h) * a.P + p), 0.f);
+        }
+        return;
+    }
+    const bool single = u.single(a.bl);
+    const int pieces = single && a.ht ? 3 : XP;
+    const int64_t pn = (int64_t)a.P * a.N;
+    const float* enter = single ? (a.h0 ? a.h0 + ((int64_t)u.seq * a.H + h) * pn : nullptr) : a.blk + ((int64_t)blockIdx.x * a.H + h) * pn;
+    float st[StateMap<NP, PT>::CT][2][4];
+    each_state<NP, PT>(st, [&](int p, int n, float& v) { v = enter && p0 + p < a.P && n < a.N ? enter[(int64_t)(p0 + p) * a.N + n] : 0.f; });
+    const float Dh = a.D ? a.D[h] : 0.f;
+    for (int i = threadIdx.x; i < PT; i += THREADS) s.bad[i] = Q;
+
+    for (int64_t t = u.t0; t < u.t1; t += Q) {
+        const int n = (int)min((int64_t)Q, u.t1 - t);
+        const bool last = t + Q >= u.t1;
+        __syncthreads();
+        chunk_steps(a, s, t, n, h);
+        load_tile<DT, XP, NP, false>(s.B[0], Q * LN, LN, a.B, t * a.b_tok + grp * a.b_grp, a.b_tok, n, a.N, a.vec, nullptr);
+        load_tile<DT, XP, NP, false>(s.C[0], Q * LN, LN, a.C, t * a.c_tok + grp * a.c_grp, a.c_tok, n, a.N, a.vec, nullptr);
+        load_tile<DT, XP, PT, true>(s.x[0], Q * LP, LP, a.x, t * a.x_tok + h * a.x_head + p0, a.x_tok, n, a.P - p0, a.vec, s.bad);
+        each_state<NP, PT>(st, [&](int p, int nn, float v) {
+            const __nv_bfloat16 hi = __float2bfloat16_rn(v);
+            s.S[0][p * LN + nn] = hi;
+            if (XP > 1) s.S[XP - 1][p * LN + nn] = __float2bfloat16_rn(v - __bfloat162float(hi));
+        });
+        __syncthreads();
+        if (!last || a.ht) scale_x(s, pieces);
+
+        // rows 16 warp .. +15: what the state gives them, e^{G_i} C_i S^T
+        const int m0 = 16 * warp;
+        const float gi[2] = {s.G[m0 + g], s.G[m0 + g + 8]};
+        float acc[PT / 8][4] = {};
+#pragma unroll
+        for (int cp = XP - 1; cp >= 0; --cp)
+#pragma unroll
+            for (int sp = XP - 1 - cp; sp >= 0; --sp)
+                warp_gemm<PT / 8, NP, false, false>(acc, s.C[cp], LN, m0, s.S[sp], LN, 0, lane);
+        {
+            const float e0 = __expf(gi[0]), e1 = __expf(gi[1]);
+#pragma unroll
+            for (int j = 0; j < PT / 8; ++j) { acc[j][0] *= e0; acc[j][1] *= e0; acc[j][2] *= e1; acc[j][3] *= e1; }
+        }
+        // and the tokens of the chunk up to their own: 16 columns of scores at a time
+#pragma unroll 1
+        for (int j0 = 0; j0 <= m0; j0 += 16) {
+            float sc[2][4] = {};
+#pragma unroll
+            for (int cp = XP - 1; cp >= 0; --cp)
+#pragma unroll
+                for (int bp = XP - 1 - cp; bp >= 0; --bp)
+                    warp_gemm<2, NP, false, false>(sc, s.C[cp], LN, m0, s.B[bp], LN, j0, lane);
+            uint32_t pa[XP][4];
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    float v[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const int i = m0 + g + 8 * r, j = j0 + 8 * c + t2 + k;
+                        v[k] = j <= i ? sc[c][2 * r + k] * __expf(gi[r] - s.G[j]) * s.d[j] : 0.f;
+                    }
+                    const uint32_t w = pack_bf16x2(v[0], v[1]);
+                    pa[0][2 * c + r] = w;
+                    if (XP > 1) {
+                        const float2 f = unpack_bf16x2(w);
+                        pa[XP - 1][2 * c + r] = pack_bf16x2(v[0] - f.x, v[1] - f.y);
+                    }
+                }
+#pragma unroll
+            for (int nt = 0; nt < PT / 8; nt += 2)
+#pragma unroll
+                for (int xp = XP - 1; xp >= 0; --xp) {
+                    uint32_t b[4];
+                    load_b_t(b, s.x[xp], LP, 8 * nt, j0, lane);
+#pragma unroll
+                    for (int pp = XP - 1 - xp; pp >= 0; --pp) {
+                        mma16816(acc[nt], pa[pp], b[0], b[1]);
+                        mma16816(acc[nt + 1], pa[pp], b[2], b[3]);
+                    }
+                }
+        }
+        // D x, gate, store
+#pragma unroll
+        for (int j = 0; j < PT / 8; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int i = m0 + g + 8 * (q >> 1), p = 8 * j + t2 + (q & 1);
+                if (i >= n || p0 + p >= a.P) continue;
+                float xv = __bfloat162float(s.x[0][i * LP + p]);
+                if (XP > 1) xv += __bfloat162float(s.x[XP - 1][i * LP + p]);
+                float v = fmaf(Dh, xv, acc[j][q]);
+                if (i >= s.bad[p]) v = __int_as_float(0x7fc00000);
+                if (a.z) {
+                    const float zv = load16<DT>(a.z, (t + i) * a.z_tok + h * a.z_head + p0 + p);
+                    v *= zv * sigmoidf_(zv);
+                }
+                Elem<DT>::st(a.y, (size_t)(((t + i) * a.H + h) * a.P + p0 + p), v);
+            }
+        if (last && !(single && a.ht)) break;
+        __syncthreads();
+        update_state(st, s, expf(s.G[Q - 1]), pieces);
+        each_state<NP, PT>(st, [&](int p, int, float& v) { if (s.bad[p] < Q) v = __int_as_float(0x7fc00000); });
+    }
+    if (single && a.ht) {
+        float* out = a.ht + ((int64_t)u.seq * a.H + h) * pn;
+        each_state<NP, PT>(st, [&](int p, int n, float v) {
+            if (p0 + p < a.P && n < a.N) out[(int64_t)(p0 + p) * a.N + n] = v;
+        });
+    }
+}
+
+template <int DT, int NP, int PT>
+int launch_np(const SsmArgs& a, int units, bool blocks, cudaStream_t st) {
+    static std::atomic<uint64_t> ready_s{0}, ready_o{0};
+    const int smem = (int)sizeof(Sm<DT, NP, PT>);
+    static_assert(sizeof(Sm<DT, NP, PT>) <= MAX_SMEM, "tiles fit");
+    const dim3 grid(units, a.H, (a.P + PT - 1) / PT);
+    if (blocks) {
+        if (!allow_smem(ready_s, ssm_state_kernel<DT, NP, PT>, smem)) return LAMPA_ERR_CUDA;
+        {
+            ProfScope prof("ssm_state", st);
+            if (launch_chained(ssm_state_kernel<DT, NP, PT>, grid, dim3(THREADS), smem, st, a) != cudaSuccess) return LAMPA_ERR_CUDA;
+        }
+    }
+    if (blocks || (a.cu && a.ht)) {
+        const int64_t slabs = ((int64_t)a.P * a.N + 255) / 256;
+        if (slabs * a.nseq > INT32_MAX) return LAMPA_ERR_UNSUPPORTED;
+        ProfScope prof("ssm_pass", st);
+        if (launch_chained(ssm_pass_kernel, dim3((unsigned)(slabs * a.nseq), a.H), dim3(256), 0, st, a) != cudaSuccess) return LAMPA_ERR_CUDA;
+    }
+    if (!allow_smem(ready_o, ssm_out_kernel<DT, NP, PT>, smem)) return LAMPA_ERR_CUDA;
+    ProfScope prof("ssm_out", st);
+    return launch_chained(ssm_out_kernel<DT, NP, PT>, grid, dim3(THREADS), smem, st, a) == cudaSuccess ? LAMPA_OK : LAMPA_ERR_CUDA;
+}
+
+template <int DT, int NP>
+int launch_dt(const SsmArgs& a, int units, bool blocks, cudaStream_t st) {
+    if (a.P <= 16) return launch_np<DT, NP, 16>(a, units, blocks, st);
+    if (a.P <= 32 || NP == 256) return launch_np<DT, NP, 32>(a, units, blocks, st);
+    if constexpr (NP < 256) return launch_np<DT, NP, 64>(a, units, blocks, st);
+    return LAMPA_ERR_UNSUPPORTED;
+}
+
+template <int DT>
+int launch_any(const SsmArgs& a, int units, bool blocks, cudaStream_t st) {
+    if (a.N <= 16) return launch_dt<DT, 16>(a, units, blocks, st);
+    if (a.N <= 32) return launch_dt<DT, 32>(a, units, blocks, st);
+    if (a.N <= 64) return launch_dt<DT, 64>(a, units, blocks, st);
+    if (a.N <= 128) return launch_dt<DT, 128>(a, units, blocks, st);
+    return launch_dt<DT, 256>(a, units, blocks, st);
+}
+
+}  // namespace
+
+int launch_ssm_scan_mma(const SsmArgs& a, int dtype, int units, bool blocks, cudaStream_t st) {
+    return dtype == LAMPA_BF16 ? launch_any<LAMPA_BF16>(a, units, blocks, st) : launch_any<LAMPA_F16>(a, units, blocks, st);
+}
+
+}  // namespace lampa

@@ -5,7 +5,8 @@ Same names and argument meaning as the reference:
   compute_lambda                         models/hattention/modeling_h_gated_deltanet.py:151-166
   FusedRMSNormGated / rms_norm_gated     models/hattention/fused_norm.py:1003-1064, 858-880
 plus `gate_inputs`, the three statements that turn the a/b/l projections into g, beta and lambda
-(modeling_h_gated_deltanet.py:429-450) as one call.  Forward only; everything runs in the CUDA
+(modeling_h_gated_deltanet.py:429-450) as one call, `short_conv`, the convolution of sequences that continue from a cache, and
+`block_norm`, the norms before and after a block with its gate and residual scale.  Forward only; everything runs in the CUDA
 library on the current stream.
 """
 from __future__ import annotations
@@ -210,6 +211,122 @@ def add_rms_norm(res: torch.Tensor, delta: Optional[torch.Tensor], weight: Optio
                                    L.ptr(L.status_word(dev)), L.stream_ptr(dev))
     L.check(rc, "lampa_add_rmsnorm")
     return y
+
+
+def short_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = "silu",
+               cache: Optional[torch.Tensor] = None, output_final_state: bool = False,
+               cu_seqlens: Optional[torch.LongTensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Depthwise causal convolution over the tokens of x [B,T,D] for sequences that continue: what lies before a sequence's first
+    token is what its cache [N,D,W] holds (W last inputs, as ShortConvolution keeps them; None: zeros).  With output_final_state
+    the cache, or a new one, becomes the last W inputs of each sequence, in place, and is returned; that of an empty sequence
+    stays.  weight: [D,W] or [D,1,W], W from 2 to 8; bias: [D]; cu_seqlens: [N+1] with B == 1 (rows behind its last entry come out
+    as zero).  x may be a part of wider rows.  Returns (y [B,T,D] in x's dtype, cache or None)."""
+    from .gated_delta import _check_cu_seqlens, _forward_only, _launched
+    from .state_space import _conv_params, _rows
+    if activation not in (None, "silu", "swish"):
+        raise ValueError(f"Activation `{activation}` not supported yet.")
+    silu = activation is not None
+    if (cache is not None or not output_final_state) and (cu_seqlens is None or cu_seqlens.is_cuda):
+        r = L.native.conv_resume(x, weight, bias, cache, cu_seqlens, silu, bool(output_final_state), True)
+        if r is not None:
+            return r, (cache if output_final_state else None)
+    _forward_only(x, weight, bias, cache)
+    if x.dim() != 3 or weight.dim() < 2:
+        raise ValueError("x [B,T,D] and weight [D,W] expected")
+    B, T, D = x.shape
+    W = weight.shape[-1]
+    dev = L.require_cuda(x, weight, bias, cache)
+    for t in (x, weight):
+        L.dtype_code(t.dtype)
+    if not 2 <= W <= 8:
+        raise NotImplementedError("convolutions of other than 2 to 8 taps are not supported")
+    w, b = _conv_params(weight, bias, D, W)
+    if cu_seqlens is not None:
+        if B != 1:
+            raise ValueError(f"The batch size is expected to be 1 rather than {B} when using `cu_seqlens`.")
+        if cu_seqlens.dim() != 1 or len(cu_seqlens) < 2:
+            raise ValueError("cu_seqlens must be a vector of at least two offsets")
+        _check_cu_seqlens(cu_seqlens, T)
+        cu_seqlens = cu_seqlens.to(device=dev, dtype=torch.int64).contiguous()
+    N = B if cu_seqlens is None else len(cu_seqlens) - 1
+    if cache is not None and (tuple(cache.shape) != (N, D, W) or not cache.is_contiguous() or cache.dtype != x.dtype):
+        raise ValueError(f"cache must be a contiguous [{N}, {D}, {W}] tensor of x's dtype")
+    if cache is None and output_final_state:
+        cache = torch.zeros(N, D, W, dtype=x.dtype, device=dev)
+    if B * T * D == 0:
+        return torch.empty(B, T, D, dtype=x.dtype, device=dev), (cache if output_final_state else None)
+    with torch.no_grad():
+        y = _launched(L.native.conv_resume(_rows(x), w, b, cache, cu_seqlens, silu, bool(output_final_state), False), "lampa_short_conv_resume")
+    return y, (cache if output_final_state else None)
+
+
+_GATE_ACTS = {None: 0, "sigmoid": 1, "silu": 2, "swish": 2}
+
+
+def block_norm(res: torch.Tensor, delta: Optional[torch.Tensor], post_weight: Optional[torch.Tensor] = None,
+               pre_weight: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, scale=None,
+               gate_activation: Optional[str] = None, eps: float = 1e-6, cu_seqlens: Optional[torch.LongTensor] = None,
+               post_norm: bool = True, out_dtype: Optional[torch.dtype] = torch.bfloat16) -> Optional[torch.Tensor]:
+    """Norms before and after a block on its fp32 residual stream `res` [rows,D], in place and in one pass:
+        res += scale * act(gate) * rms_norm(delta) * post_weight        (post_norm False: delta itself)
+        y = rms_norm(res) * pre_weight                                  (the next block's input, in out_dtype)
+    delta [rows,D]: the block's output (None: the norm only).  gate: [rows,D], [D], or with cu_seqlens [N+1] one row [N,D] per
+    sequence (a row of no sequence keeps its residual); gate_activation None, "sigmoid" or "silu".  scale: None, a number or [D].
+    Weights [D] or None.  out_dtype None: no norm behind the update (returns None).  D up to 8192."""
+    from .gated_delta import _check_cu_seqlens, _forward_only, _launched
+    if gate_activation not in _GATE_ACTS:
+        raise ValueError(f"Unsupported activation: {gate_activation}")
+    act, ydt = _GATE_ACTS[gate_activation], -1 if out_dtype is None else L.dtype_code(out_dtype)
+    is_tensor = isinstance(scale, torch.Tensor)
+    number = scale if is_tensor else 1.0 if scale is None else float(scale)
+    if cu_seqlens is None or cu_seqlens.is_cuda:
+        r = L.native.block_norm(res, delta, post_weight, pre_weight, gate, number, act, float(eps), cu_seqlens, bool(post_norm), ydt, True)
+        if r is not None:
+            return None if r is True else r
+    _forward_only(res, delta, post_weight, pre_weight, gate, scale if is_tensor else None)
+    if res.dim() != 2 or res.dtype != torch.float32 or not res.is_contiguous():
+        raise ValueError("res must be a contiguous fp32 [rows, D] tensor (updated in place)")
+    rows, D = res.shape
+    dev = L.require_cuda(res, delta, post_weight, pre_weight, gate, scale if is_tensor else None)
+    if delta is None and (gate is not None or out_dtype is None):
+        raise ValueError("without delta there is the norm of res only")
+    if delta is not None and tuple(delta.shape) != (rows, D):
+        raise ValueError("delta must match res")
+    if cu_seqlens is not None and gate is None:
+        raise ValueError("cu_seqlens says which sequence's gate a row takes: gate is missing")
+    if D > 8192:
+        raise NotImplementedError("rows of more than 8192 elements are not supported")
+    vec = lambda t, n: None if t is None else _vector(t, D, n)  # noqa: E731
+    post_weight, pre_weight = vec(post_weight, "post_weight"), vec(pre_weight, "pre_weight")
+    if is_tensor:
+        number = vec(scale, "scale")
+    if cu_seqlens is not None:
+        if cu_seqlens.dim() != 1 or len(cu_seqlens) < 2:
+            raise ValueError("cu_seqlens must be a vector of at least two offsets")
+        _check_cu_seqlens(cu_seqlens, rows)
+        cu_seqlens = cu_seqlens.to(device=dev, dtype=torch.int64).contiguous()
+    if gate is not None:
+        n = rows if cu_seqlens is None else len(cu_seqlens) - 1
+        if gate.dim() == 1 or (gate.dim() == 2 and gate.shape[0] == 1):
+            gate = gate.expand(n, gate.shape[-1])
+        if tuple(gate.shape) != (n, D):
+            raise ValueError(f"gate must be [{n}, {D}] or [{D}]")
+    for t in (delta, gate):
+        if t is not None:
+            L.dtype_code(t.dtype)
+    if rows * D == 0:
+        return None if out_dtype is None else torch.empty(rows, D, dtype=out_dtype, device=dev)
+    last = lambda t: t if t is None or D <= 1 or t.stride(-1) == 1 else t.contiguous()  # noqa: E731
+    with torch.no_grad():
+        r = _launched(L.native.block_norm(res, last(delta), post_weight, pre_weight, last(gate), number, act, float(eps), cu_seqlens,
+                                          bool(post_norm), ydt, False), "lampa_block_norm")
+    return None if r is True else r
+
+
+def _vector(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
+    if tuple(t.shape) != (n,):
+        raise ValueError(f"{name} must be [{n}]")
+    return t.detach().to(torch.float32).contiguous()
 
 
 class FusedRMSNormGated(nn.Module):
