@@ -153,6 +153,7 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 // is left unbalanced.  A thread that has given up once (`dead`) does not wait again: it runs to the
 // end of its loop, issues nothing new and drains what it has in flight with mbar_drain.
 constexpr int MBAR_POLLS = 1 << 22;
+bool umma_enabled();               // false on the mma.sync twins (lampa_debug_force_mma_sync, LAMPA_B200_NO_UMMA=1)
 int poll_budget();                 // of the launches that follow (host): MBAR_POLLS unless lampa_debug_set_poll_budget lowered it
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, bool& dead, int32_t* status, int where, int budget) {
     if (dead) return false;

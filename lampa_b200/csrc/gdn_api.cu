@@ -8,13 +8,17 @@ using namespace lampa;
 namespace lampa {
 static int g_poll_budget = MBAR_POLLS;
 int poll_budget() { return g_poll_budget; }
+static int g_force_mma_sync = 0;  // see lampa_debug_force_mma_sync
+bool umma_enabled() {
+    static const bool off = [] { const char* e = getenv("LAMPA_B200_NO_UMMA"); return e && e[0] == '1'; }();
+    return !off && !g_force_mma_sync;
+}
 }  // namespace lampa
 
 namespace {
 
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
-int g_force_mma_sync = 0;         // see lampa_debug_force_mma_sync
 long long* g_ticks = nullptr;     // see lampa_debug_set_tick_buffer
 int g_ticks_ctas = 0;
 
@@ -103,8 +107,7 @@ void fill_args(const lampa_gdn_desc* d, bool hier, const Layout& l, char* base, 
     a.blk = base + l.off_blk;
     a.entry = (float*)(base + l.off_entry);
     a.status = status;
-    static const int no_umma = [] { const char* e = getenv("LAMPA_B200_NO_UMMA"); return (e && e[0] == '1') ? 1 : 0; }();
-    a.use_umma = (no_umma || g_force_mma_sync) ? 0 : 1;
+    a.use_umma = umma_enabled() ? 1 : 0;
     a.poll_budget = poll_budget();
     a.long_only = a.short_only = 0;
     a.signal = 0;

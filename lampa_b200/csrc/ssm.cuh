@@ -15,7 +15,7 @@ struct SsmArgs {
     const int64_t* cu;
     void* y; float* ht;
     float* blk;                       // [units][H][P][N]: end states of blocks that begin empty, then the states that enter them
-    float* blk_dec;                   // [units][H]: log decay of a block
+    float* blk_dec;                   // [units][H]: log2 of a block's decay
     int32_t* status;
     int64_t x_tok, x_head, z_tok, z_head, b_tok, b_grp, c_tok, c_grp, dt_tok;   // distances in elements
     int64_t n_tok, T;                 // rows in all; tokens per sequence without cu
@@ -23,7 +23,8 @@ struct SsmArgs {
     int nb;                           // blocks per sequence without cu
     int bl;                           // tokens per block
     int H, P, N, G, dt_dt, softplus;
-    int vec;                          // rows of x, B and C are 16-byte aligned
+    int vec, z_vec;                   // rows of x, B and C, or of z, are 16-byte aligned
+    int whole;                        // the block kernel also has the states of sequences of one block (tcgen05 form)
     int poll_budget;
 };
 
@@ -71,6 +72,8 @@ __device__ __forceinline__ float ssm_step_size(float v, int softplus) {
     return softplus ? fmaxf(v, 0.f) + log1pf(expf(-fabsf(v))) : v;
 }
 
+int launch_ssm_pass(const SsmArgs& a, cudaStream_t st);
+int launch_ssm_scan_umma(const SsmArgs& a, int units, bool blocks, cudaStream_t st);
 int launch_ssm_scan_mma(const SsmArgs& a, int dtype, int units, bool blocks, cudaStream_t st);
 
 }  // namespace lampa

@@ -15,23 +15,28 @@ bool built(const lampa_ssm_desc* d) {
     return (d->dtype == LAMPA_BF16 || d->dtype == LAMPA_F16) && d->N <= 256 && d->H <= 65535 && d->P <= 65535;
 }
 
-// Tokens per block: enough blocks for six CTAs to an SM.
-int block_tokens(const lampa_ssm_desc* d) {
-    const int64_t n_tok = (int64_t)d->B * d->T, chunks = (n_tok + SSM_Q - 1) / SSM_Q;
-    const int64_t per = (int64_t)d->H * ((d->P + 63) / 64), want = std::max<int64_t>(1, 6 * sm_count() / per);
-    return (int)std::min<int64_t>(1 << 20, std::max<int64_t>(2, (chunks + want - 1) / want)) * SSM_Q;
+// The tcgen05 kernels take bf16 rows in pieces of 16 bytes, and their state is one operand tile.
+bool umma_shape(const lampa_ssm_desc* d) { return d->dtype == LAMPA_BF16 && d->P % 8 == 0 && d->N % 8 == 0 && d->N <= 128; }
+
+// Tokens per block.  mma.sync: enough blocks for six CTAs to an SM; tcgen05: for one CTA (of two heads) to an SM.
+int block_tokens(const lampa_ssm_desc* d, bool umma) {
+    const int q = umma ? 128 : SSM_Q;
+    const int64_t n_tok = (int64_t)d->B * d->T, chunks = (n_tok + q - 1) / q, slabs = (d->P + 63) / 64;
+    const int64_t per = umma ? (int64_t)d->G * ((d->H / d->G + 1) / 2) * slabs : d->H * slabs;
+    const int64_t want = std::max<int64_t>(1, (umma ? 1 : 6) * sm_count() / per);
+    return (int)std::min<int64_t>(1 << 20, std::max<int64_t>(umma ? 1 : 2, (chunks + want - 1) / want)) * q;
 }
 
 struct Plan { int bl, nb; int64_t units; bool blocks; size_t state_bytes, bytes; };
-Plan plan_of(const lampa_ssm_desc* d) {
+Plan plan_of(const lampa_ssm_desc* d, bool umma) {
     Plan p;
     const int64_t n_tok = (int64_t)d->B * d->T;
-    p.bl = block_tokens(d);
+    p.bl = block_tokens(d, umma);
     p.nb = (int)(((int64_t)d->T + p.bl - 1) / p.bl);
     p.units = ssm_units(n_tok, d->nseq ? d->nseq : d->B, p.nb, p.bl, d->nseq > 0);
     p.blocks = d->T > p.bl;                                        // some sequence may have more than one
     p.state_bytes = (size_t)p.units * d->H * d->P * d->N * 4;
-    p.bytes = p.blocks ? p.state_bytes + (size_t)p.units * d->H * 4 : 0;
+    p.bytes = p.blocks || umma ? p.state_bytes + (size_t)p.units * d->H * 4 : 0;
     return p;
 }
 
@@ -43,7 +48,8 @@ using namespace lampa;
 extern "C" int lampa_ssm_workspace_bytes(const lampa_ssm_desc* d, size_t* bytes) {
     if (!desc_ok(d) || !bytes) return LAMPA_ERR_ARG;
     if (!built(d)) return LAMPA_ERR_UNSUPPORTED;
-    *bytes = d->B && d->T ? plan_of(d).bytes : 0;
+    *bytes = 0;
+    if (d->B && d->T) *bytes = std::max(plan_of(d, false).bytes, umma_shape(d) ? plan_of(d, true).bytes : 0);
     return LAMPA_OK;
 }
 
@@ -56,9 +62,12 @@ extern "C" int lampa_ssm_scan(const lampa_ssm_desc* d, const void* x, int64_t x_
     if (!built(d)) return LAMPA_ERR_UNSUPPORTED;
     if (d->B == 0 || d->T == 0) return LAMPA_OK;
     if (!x || !dt || !A || !B || !C || !y) return LAMPA_ERR_ARG;
-    const Plan p = plan_of(d);
+    auto rows16 = [](const void* q, int64_t s0, int64_t s1) { return (((uintptr_t)q | (uintptr_t)(s0 * 2) | (uintptr_t)(s1 * 2)) & 15) == 0; };
+    const bool vec = d->P % 8 == 0 && d->N % 8 == 0 && rows16(x, x_tok, x_head) && rows16(B, b_tok, b_grp) && rows16(C, c_tok, c_grp);
+    const bool umma = umma_shape(d) && vec && ((uintptr_t)y & 15) == 0 && umma_enabled();
+    const Plan p = plan_of(d, umma);
     if (p.units > INT32_MAX) return LAMPA_ERR_UNSUPPORTED;
-    if (p.blocks && (!ws || ws_bytes < p.bytes || ((uintptr_t)ws & 15))) return LAMPA_ERR_WORKSPACE;
+    if (p.bytes && (!ws || ws_bytes < p.bytes || ((uintptr_t)ws & 15))) return LAMPA_ERR_WORKSPACE;
     SsmArgs a = {};
     a.x = x; a.dt = dt; a.B = B; a.C = C; a.z = z;
     a.A = A; a.D = D; a.dt_bias = dt_bias; a.h0 = initial_state; a.cu = cu_seqlens;
@@ -69,8 +78,9 @@ extern "C" int lampa_ssm_scan(const lampa_ssm_desc* d, const void* x, int64_t x_
     a.dt_tok = dt_tok;
     a.n_tok = (int64_t)d->B * d->T; a.T = d->T; a.nseq = d->nseq ? d->nseq : d->B; a.nb = p.nb; a.bl = p.bl;
     a.H = d->H; a.P = d->P; a.N = d->N; a.G = d->G; a.dt_dt = d->dt_dtype; a.softplus = d->dt_softplus;
-    auto rows16 = [](const void* q, int64_t s0, int64_t s1) { return (((uintptr_t)q | (uintptr_t)(s0 * 2) | (uintptr_t)(s1 * 2)) & 15) == 0; };
-    a.vec = d->P % 8 == 0 && d->N % 8 == 0 && rows16(x, x_tok, x_head) && rows16(B, b_tok, b_grp) && rows16(C, c_tok, c_grp);
+    a.vec = vec;
+    a.z_vec = z && rows16(z, z_tok, z_head);
+    a.whole = umma;
     a.poll_budget = poll_budget();
-    return launch_ssm_scan_mma(a, d->dtype, (int)p.units, p.blocks, (cudaStream_t)stream);
+    return umma ? launch_ssm_scan_umma(a, (int)p.units, p.blocks, (cudaStream_t)stream) : launch_ssm_scan_mma(a, d->dtype, (int)p.units, p.blocks, (cudaStream_t)stream);
 }

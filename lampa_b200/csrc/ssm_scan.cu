@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(THREADS) ssm_state_kernel(SsmArgs a) {
         __syncthreads();
         const float g = s.G[Q - 1];
         update_state(st, s, expf(g), 3);
-        log_dec += g;
+        log_dec += g * 1.4426950408889634f;
     }
     float* out = a.blk + ((int64_t)blockIdx.x * a.H + h) * a.P * a.N;
     each_state<NP, PT>(st, [&](int p, int n, float v) {
@@ -232,14 +232,14 @@ __global__ void __launch_bounds__(256) ssm_pass_kernel(SsmArgs a) {
     if (e >= pn) return;
     const int64_t len = eos - bos, out = ((int64_t)seq * a.H + h) * pn + e;
     float s = a.h0 ? a.h0[out] : 0.f;
-    if (len > a.bl) {
+    if (len > a.bl || (a.whole && a.ht && len > 0)) {
         const int nb = (int)((len + a.bl - 1) / a.bl);
         float* p = a.blk + (u0 * a.H + h) * pn + e;
         const float* dec = a.blk_dec + u0 * a.H + h;
         for (int b = 0; b < nb; ++b) {
             const float part = *p;
             *p = s;
-            s = fmaf(expf(*dec), s, part);
+            s = fmaf(exp2f(*dec), s, part);
             p += (int64_t)a.H * pn;
             dec += a.H;
         }
@@ -392,10 +392,8 @@ int launch_np(const SsmArgs& a, int units, bool blocks, cudaStream_t st) {
         }
     }
     if (blocks || (a.cu && a.ht)) {
-        const int64_t slabs = ((int64_t)a.P * a.N + 255) / 256;
-        if (slabs * a.nseq > INT32_MAX) return LAMPA_ERR_UNSUPPORTED;
-        ProfScope prof("ssm_pass", st);
-        if (launch_chained(ssm_pass_kernel, dim3((unsigned)(slabs * a.nseq), a.H), dim3(256), 0, st, a) != cudaSuccess) return LAMPA_ERR_CUDA;
+        const int rc = launch_ssm_pass(a, st);
+        if (rc != LAMPA_OK) return rc;
     }
     if (!allow_smem(ready_o, ssm_out_kernel<DT, NP, PT>, smem)) return LAMPA_ERR_CUDA;
     ProfScope prof("ssm_out", st);
@@ -420,6 +418,13 @@ int launch_any(const SsmArgs& a, int units, bool blocks, cudaStream_t st) {
 }
 
 }  // namespace
+
+int launch_ssm_pass(const SsmArgs& a, cudaStream_t st) {
+    const int64_t slabs = ((int64_t)a.P * a.N + 255) / 256;
+    if (slabs * a.nseq > INT32_MAX) return LAMPA_ERR_UNSUPPORTED;
+    ProfScope prof("ssm_pass", st);
+    return launch_chained(ssm_pass_kernel, dim3((unsigned)(slabs * a.nseq), a.H), dim3(256), 0, st, a) == cudaSuccess ? LAMPA_OK : LAMPA_ERR_CUDA;
+}
 
 int launch_ssm_scan_mma(const SsmArgs& a, int dtype, int units, bool blocks, cudaStream_t st) {
     return dtype == LAMPA_BF16 ? launch_any<LAMPA_BF16>(a, units, blocks, st) : launch_any<LAMPA_F16>(a, units, blocks, st);

@@ -30,12 +30,16 @@ def _head_vector(t: Optional[torch.Tensor], H: int, name: str, dev) -> Optional[
     return t.detach().to(device=dev, dtype=torch.float32).contiguous()
 
 
-def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    """t [B, T, ...] itself where its tokens lie one distance apart and its last axis is contiguous, else a dense copy."""
+def _rows(t: Optional[torch.Tensor], aligned: bool = False) -> Optional[torch.Tensor]:
+    """t [B, T, ...] itself where its tokens lie one distance apart and its last axis is contiguous (`aligned`: and every row of
+    it begins on a 16-byte boundary), else a dense copy."""
     if t is None:
         return None
     even = t.shape[0] <= 1 or t.shape[1] <= 1 or t.stride(0) == t.shape[1] * t.stride(1)
-    return t if even and (t.shape[-1] <= 1 or t.stride(-1) == 1) else t.contiguous()
+    even = even and (t.shape[-1] <= 1 or t.stride(-1) == 1)
+    if aligned:
+        even = even and not any(v * t.element_size() % 16 for v in t.stride()[:-1]) and t.data_ptr() % 16 == 0
+    return t if even else t.contiguous()
 
 
 def state_space_scan(
@@ -57,7 +61,8 @@ def state_space_scan(
     x, z: [B,T,H,P]; dt: [B,T,H]; B, C: [B,T,G,N] with G dividing H; A, D, dt_bias: [H]; initial_state: [N_seq,H,P,N]
     (not changed); cu_seqlens: [N_seq+1] with B == 1.  Returns (y [B,T,H,P] in x's dtype, final state [N_seq,H,P,N] fp32 or
     None).  x, B, C and z are bf16 or fp16 (fp32 is refused: the products run on 16-bit operands) and may be parts of wider
-    rows, as a projection's output is split; dt may have a type of its own.  Any P, N up to 256, any lengths from 0 on; rows
+    rows, as a projection's output is split (x, B and C are copied where these do not begin on 16-byte boundaries); dt may
+    have a type of its own.  Any P, N up to 256, any lengths from 0 on; rows
     behind the last entry of cu_seqlens come out as zero.  D None: no skip; z None: no gate.
     The last bits of y and of the states depend on how long the whole call is (the tokens are cut into blocks), those of two
     equal calls do not differ.
@@ -100,8 +105,9 @@ def state_space_scan(
             ht = initial_state.clone() if initial_state is not None else torch.zeros(nseq, H, P, N, device=dev)
         return torch.empty(Bn, T, H, P, dtype=x.dtype, device=dev), ht
     A, D, dt_bias = (_head_vector(t, H, n, dev) for t, n in ((A, "A"), (D, "D"), (dt_bias, "dt_bias")))
+    wide = P % 8 == 0 and N % 8 == 0              # rows of whole 16-byte pieces: the kernels read them as such
     with torch.no_grad():
-        return _launched(L.native.ssm_scan(_rows(x), _rows(dt), A, _rows(B), _rows(C), D, _rows(z), dt_bias, initial_state,
+        return _launched(L.native.ssm_scan(_rows(x, wide), _rows(dt), A, _rows(B, wide), _rows(C, wide), D, _rows(z), dt_bias, initial_state,
                                            cu_seqlens, bool(dt_softplus), bool(output_final_state), False), "lampa_ssm_scan")
 
 

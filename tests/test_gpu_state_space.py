@@ -81,6 +81,22 @@ def test_scan_over_blocks(lb, dtype, P, N, H, G):
         check_scan(lb, scan_inputs(int(decay * 10), 1, 3001, H, P, G, N, dtype, z=True, h0=True, decay=decay))
 
 
+@pytest.mark.parametrize("P,N,H,G,T", [(64, 128, 4, 1, 1300), (64, 64, 6, 2, 700), (40, 72, 5, 1, 515), (136, 128, 3, 3, 260), (8, 8, 2, 1, 400), (64, 120, 1, 1, 129)])
+def test_scan_kernels_agree(lb, P, N, H, G, T):
+    """The tcgen05 kernels and their mma.sync twins on one input, each within its bound of the recurrence"""
+    from lampa_b200 import _lib
+    for pitch in (0, 8):
+        a = scan_inputs(T, 2, T, H, P, G, N, BF, z=True, h0=True, pitch=pitch)
+        try:
+            for off in (0, 1):
+                _lib.lib().lampa_debug_force_mma_sync(off)
+                check_scan(lb, a)
+        finally:
+            _lib.lib().lampa_debug_force_mma_sync(0)
+        a["z"] = torch.cat([a["z"], a["z"][..., :1]], 3)[..., :P]          # rows of z that are not 16-byte aligned
+        check_scan(lb, a)
+
+
 @pytest.mark.parametrize("dtype", [BF, FP])
 @pytest.mark.parametrize("lens", [[1], [0, 1, 63, 0, 64, 65, 200, 0], [5, 700, 0, 0, 1, 129, 1300, 2], [128, 128, 128], [0, 0, 3]])
 def test_scan_packed(lb, dtype, lens):
@@ -186,6 +202,21 @@ def test_scan_offsets_on_the_device_are_checked(lb):
     y, ht = lb.state_space_scan(**a, output_final_state=True, cu_seqlens=torch.tensor([0, 100, 100, 230], device="cuda"))
     lb.check_status()
     assert (y[0, 230:] == 0).all() and (ht[1] == 0).all()          # rows behind the last sequence
+
+
+def test_scan_waits_are_bounded(lb):
+    """With no polls left every wait gives up: the call ends, says so, and the next one is right"""
+    from lampa_b200 import _lib
+    a = scan_inputs(12, 1, 1000, 4, 64, 1, 128, BF, z=True, h0=True)
+    try:
+        _lib.lib().lampa_debug_set_poll_budget(0)
+        lb.state_space_scan(**a, output_final_state=True)
+        torch.cuda.synchronize()
+    finally:
+        _lib.lib().lampa_debug_set_poll_budget(1 << 22)
+    with pytest.raises(lb.LampaError):
+        lb.check_status()
+    check_scan(lb, a)
 
 
 def test_scan_in_a_graph_and_on_another_stream(lb):
