@@ -73,7 +73,7 @@ __device__ __forceinline__ float ssm_step_size(float v, int softplus) {
 }
 
 int launch_ssm_pass(const SsmArgs& a, cudaStream_t st);
-int launch_ssm_scan_umma(const SsmArgs& a, int units, bool blocks, cudaStream_t st);
+int launch_ssm_scan_umma(SsmArgs a, int units, bool blocks, cudaStream_t st);
 int launch_ssm_scan_mma(const SsmArgs& a, int dtype, int units, bool blocks, cudaStream_t st);
 
 }  // namespace lampa

@@ -64,7 +64,7 @@ extern "C" int lampa_ssm_scan(const lampa_ssm_desc* d, const void* x, int64_t x_
     if (!x || !dt || !A || !B || !C || !y) return LAMPA_ERR_ARG;
     auto rows16 = [](const void* q, int64_t s0, int64_t s1) { return (((uintptr_t)q | (uintptr_t)(s0 * 2) | (uintptr_t)(s1 * 2)) & 15) == 0; };
     const bool vec = d->P % 8 == 0 && d->N % 8 == 0 && rows16(x, x_tok, x_head) && rows16(B, b_tok, b_grp) && rows16(C, c_tok, c_grp);
-    const bool umma = umma_shape(d) && vec && ((uintptr_t)y & 15) == 0 && umma_enabled();
+    const bool umma = umma_shape(d) && (int64_t)d->B * d->T <= INT32_MAX - 128 && vec && ((uintptr_t)y & 15) == 0 && umma_enabled();
     const Plan p = plan_of(d, umma);
     if (p.units > INT32_MAX) return LAMPA_ERR_UNSUPPORTED;
     if (p.bytes && (!ws || ws_bytes < p.bytes || ((uintptr_t)ws & 15))) return LAMPA_ERR_WORKSPACE;

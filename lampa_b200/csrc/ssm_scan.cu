@@ -236,12 +236,20 @@ __global__ void __launch_bounds__(256) ssm_pass_kernel(SsmArgs a) {
         const int nb = (int)((len + a.bl - 1) / a.bl);
         float* p = a.blk + (u0 * a.H + h) * pn + e;
         const float* dec = a.blk_dec + u0 * a.H + h;
-        for (int b = 0; b < nb; ++b) {
-            const float part = *p;
-            *p = s;
-            s = fmaf(exp2f(*dec), s, part);
-            p += (int64_t)a.H * pn;
-            dec += a.H;
+        const int64_t step = (int64_t)a.H * pn;
+        for (int b = 0; b < nb; b += 8) {                          // eight blocks are asked for before the first is used
+            float part[8], e[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                part[k] = b + k < nb ? p[(b + k) * step] : 0.f;
+                e[k] = b + k < nb ? dec[(int64_t)(b + k) * a.H] : 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (b + k < nb) {
+                    p[(b + k) * step] = s;
+                    s = fmaf(exp2f(e[k]), s, part[k]);
+                }
         }
     } else if (len > 0) return;
     if (a.ht) a.ht[out] = s;

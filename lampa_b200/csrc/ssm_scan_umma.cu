@@ -5,15 +5,19 @@
 // columns to a panel, serve as either operand of every product):
 //   G   = C B^T                   128 x 128, K = N                        scores
 //   Y   = C [S_a^T | S_b^T]       128 x 128, K = N                        what the entering states give; scaled by e^{G_i} in place
-//   dS  = B^T [wx_a | wx_b]       N x 128,   K = 128 tokens               what the chunk adds to the states
+//   S  += B^T [wx_a | wx_b]       N x 128,   K = 128 tokens               what the chunk adds to the states, decayed before
 //   Y_h += P_h x_h                128 x 64 each, K = 128                  P_h: masked, decayed scores, bf16, from tensor memory
-// All accumulators are in tensor memory (G | P | Y | dS, 128 columns each).  The states stay in registers in fp32.
+// All accumulators are in tensor memory (G | P | Y | S, 128 columns each), the states S in fp32 among them.
 //
-// Sixteen warps do the element work, thread = (row or state row, head, half of the 64 columns); a control warp issues the products and is
-// the only one that polls mbarriers: it passes completions on through hardware named barriers (30 cycles, where a poll costs 200 - 300).
-// Its waits are bounded and it walks through all barriers whether or not one ran out, so nobody can be left waiting.
+// Sixteen warps do the element work, thread = (row or state row, head, half of the 64 columns).  Three more serve them.  One issues the
+// products (and is held up while the tensor core's queue is full, so that it does nothing else).  One copies the tiles in (tiled TMA from
+// three-dimensional maps, which fill what lies beyond the head's columns with zeros) and is the only one that polls for completions: it
+// passes them on through hardware named barriers (30 cycles, where a poll costs 200 - 300).  One turns the chunks' steps into decays a
+// chunk ahead.  Waits are bounded, and the helpers walk through all their barriers whether or not one ran out, so
+// nobody can be left waiting; nor can anybody reach a barrier twice in one phase, because no warp is more than a chunk ahead of another.
 #include "profile.cuh"
 #include "ssm.cuh"
+#include "tmap.cuh"
 #include "umma.cuh"
 
 #include <algorithm>
@@ -23,82 +27,96 @@ namespace {
 
 constexpr int UQ = 128;                           // tokens per chunk
 constexpr int CWARPS = 16, CT = CWARPS * 32;      // element warps
-constexpr int THREADS = CT + 32;
+constexpr int W_MMA = CWARPS, W_CTL = CWARPS + 1, W_TAB = CWARPS + 2;     // products; copies and completions; steps
+constexpr int THREADS = CT + 96;                  // (three helpers: with a fourth an element thread would have 96 registers, not 104)
 constexpr int TILE = 16384;                       // [128][64] bf16
 constexpr float LOG2E = 1.4426950408889634f;
 
 // tensor-memory columns
 constexpr int TM_G = 0, TM_P = 128, TM_Y = 256, TM_S = 384;
 
-__device__ __forceinline__ void nb_sync(int id) { asm volatile("bar.sync %0, %1;\n" :: "r"(id), "n"(THREADS) : "memory"); }
-__device__ __forceinline__ void nb_arrive(int id) { asm volatile("bar.arrive %0, %1;\n" :: "r"(id), "n"(THREADS) : "memory"); }
+// named barriers of the element warps with one helper (CC), with the copying and the step warp (CS), with everybody (ALL), and of two
+// helpers (HH)
+constexpr int CC = CT + 32, CS = CT + 64, ALL = THREADS, HH = 64;
+template <int N> __device__ __forceinline__ void nb_sync(int id) { asm volatile("bar.sync %0, %1;\n" :: "r"(id), "n"(N) : "memory"); }
+template <int N> __device__ __forceinline__ void nb_arrive(int id) { asm volatile("bar.arrive %0, %1;\n" :: "r"(id), "n"(N) : "memory"); }
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" :: "r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_all;\n" ::: "memory"); }
 __device__ __forceinline__ uint64_t adv(uint64_t d, uint32_t bytes) { return d + (uint64_t)(bytes >> 4); }
 __device__ __forceinline__ int swz(int r, int c16) { return r * 128 + ((c16 ^ (r & 7)) << 4); }
+__device__ __forceinline__ F2 unpack2(uint32_t u) { return f2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
+__device__ __forceinline__ uint32_t pack2(F2 v) { float lo, hi; f2_get(v, lo, hi); return pack_bf16x2(lo, hi); }
+
+// [128 tokens][64 columns] of one head (or group) into a panel
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t t, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n"
+                 :: "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(t), "r"(smem_u32(bar)) : "memory");
+}
 
 // Per head and chunk, by token: G (log2), d, d e^{G_end(32-block) - G}, d e^{G_last - G}
 struct Tab { float G[UQ], d[UQ], cf[UQ], w[UQ]; };
 
-// One warp, four tokens to a lane.  Returns log2 of the chunk's decay.  The exponent of w is summed from the chunk's end, so
-// that its error is one of its own size.
-__device__ __forceinline__ void raw_steps(const SsmArgs& a, int64_t t, int64_t t1, int h, bool has, float (&v)[4]) {
-    const int lane = threadIdx.x & 31;
+// One warp, four tokens to a lane, both heads; tokens from n on have d = 0.  g2: log2 of the chunk's decay.  The exponent of w is summed
+// from the chunk's end, so that its error is one of its own size.
+struct Steps { float A2[2], bias[2]; int h[2]; bool has[2]; };
+__device__ __forceinline__ Steps steps_of(const SsmArgs& a, int h0, bool second) {
+    Steps p;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int64_t i = t + 4 * lane + k;
-        v[k] = has && i < t1 ? load_as_float(a.dt, (size_t)(i * a.dt_tok + h), a.dt_dt) : 0.f;
+    for (int k = 0; k < 2; ++k) {
+        p.has[k] = k == 0 || second;
+        p.h[k] = p.has[k] ? h0 + k : h0;
+        p.A2[k] = a.A[p.h[k]] * LOG2E;
+        p.bias[k] = a.dt_bias ? a.dt_bias[p.h[k]] : 0.f;
     }
+    return p;
 }
 template <bool FULL>
-__device__ __forceinline__ float make_tab(const SsmArgs& a, float* ws, Tab* s, const float (&raw)[4], int n, float A2, float bias) {
+__device__ __forceinline__ void make_tabs(const SsmArgs& a, const Steps& p, float* const (&ws)[2], Tab* s, int64_t t, int n, float (&g2)[2]) {
     const int l = threadIdx.x & 31;
-    float d[4], g[4], up = 0.f;
+    float d[2][4], g[2][4], up[2] = {0.f, 0.f}, down[2];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        d[k] = 4 * l + k < n ? ssm_step_size(raw[k] + bias, a.softplus) : 0.f;
-        g[k] = 4 * l + k < n ? d[k] * A2 : 0.f;
-        up += g[k];
+        const int64_t at = (t + min(4 * l + k, n - 1)) * a.dt_tok;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) d[x][k] = a.dt_dt == LAMPA_F32 ? __ldg((const float*)a.dt + at + p.h[x]) : __uint_as_float((uint32_t)__ldg((const uint16_t*)a.dt + at + p.h[x]));
     }
-    float down = up;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const float u = __shfl_up_sync(0xffffffffu, up, o), v = __shfl_down_sync(0xffffffffu, down, o);
-        if (l >= o) up += u;
-        if (l + o < 32) down += v;
-    }
-    const float before = __shfl_up_sync(0xffffffffu, up, 1), after = __shfl_down_sync(0xffffffffu, down, 1);
-    float e = l < 31 ? after : 0.f, w[4];
+    for (int x = 0; x < 2; ++x)
 #pragma unroll
-    for (int k = 3; k >= 0; --k) { w[k] = d[k] * exp2f(e); e += g[k]; }
-    *reinterpret_cast<float4*>(ws + 4 * l) = make_float4(w[0], w[1], w[2], w[3]);
-    if (FULL) {
-        float G[4], b = l ? before : 0.f;
+        for (int k = 0; k < 4; ++k) {
+            float v = d[x][k];
+            if (a.dt_dt == LAMPA_BF16) v = __uint_as_float(__float_as_uint(v) << 16);
+            else if (a.dt_dt == LAMPA_F16) v = __half2float(__ushort_as_half((unsigned short)__float_as_uint(v)));
+            const bool in = 4 * l + k < n && p.has[x];
+            d[x][k] = in ? ssm_step_size(v + p.bias[x], a.softplus) : 0.f;
+            g[x][k] = in ? d[x][k] * p.A2[x] : 0.f;
+            up[x] += g[x][k];
+        }
+    down[0] = up[0]; down[1] = up[1];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) { b += g[k]; G[k] = b; }
-        const float end = __shfl_sync(0xffffffffu, G[3], l | 7);
-        *reinterpret_cast<float4*>(&s->G[4 * l]) = make_float4(G[0], G[1], G[2], G[3]);
-        *reinterpret_cast<float4*>(&s->d[4 * l]) = make_float4(d[0], d[1], d[2], d[3]);
-        *reinterpret_cast<float4*>(&s->cf[4 * l]) = make_float4(d[0] * ex2(end - G[0]), d[1] * ex2(end - G[1]), d[2] * ex2(end - G[2]), d[3] * ex2(end - G[3]));
-    }
-    return __shfl_sync(0xffffffffu, up, 31);
-}
-
-// [128] rows of PAN * 64 columns into PAN panels, zero beyond n rows and `cols` columns; by the element warps
-template <int PAN>
-__device__ __forceinline__ void load_panels(uint32_t dst, const void* base, int64_t off, int64_t pitch, int n, int cols, bool twice) {
-    const __nv_bfloat16* src = (const __nv_bfloat16*)base + off;
+    for (int o = 1; o < 32; o <<= 1)
 #pragma unroll
-    for (int k = 0; k < UQ * 8 * PAN / CT; ++k) {
-        const int i = threadIdx.x + CT * k, r = i / (8 * PAN), c = i % (8 * PAN);
-        const bool ok = r < n && c * 8 < cols;
-        const uint32_t at = dst + (c >> 3) * TILE + swz(r, c & 7);
-        const void* p = ok ? src + (int64_t)r * pitch + c * 8 : src;
-        cp16(at, p, ok);
-        if (PAN == 1 && twice) cp16(at + TILE, p, ok);
+        for (int x = 0; x < 2; ++x) {
+            const float u = __shfl_up_sync(0xffffffffu, up[x], o), v = __shfl_down_sync(0xffffffffu, down[x], o);
+            if (l >= o) up[x] += u;
+            if (l + o < 32) down[x] += v;
+        }
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const float before = __shfl_up_sync(0xffffffffu, up[x], 1), after = __shfl_down_sync(0xffffffffu, down[x], 1);
+        float e = l < 31 ? after : 0.f, w[4];
+#pragma unroll
+        for (int k = 3; k >= 0; --k) { w[k] = d[x][k] * exp2f(e); e += g[x][k]; }
+        *reinterpret_cast<float4*>(ws[x] + 4 * l) = make_float4(w[0], w[1], w[2], w[3]);
+        if (FULL) {
+            float G[4], b = l ? before : 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { b += g[x][k]; G[k] = b; }
+            const float end = __shfl_sync(0xffffffffu, G[3], l | 7);
+            *reinterpret_cast<float4*>(&s[x].G[4 * l]) = make_float4(G[0], G[1], G[2], G[3]);
+            *reinterpret_cast<float4*>(&s[x].d[4 * l]) = make_float4(d[x][0], d[x][1], d[x][2], d[x][3]);
+            *reinterpret_cast<float4*>(&s[x].cf[4 * l]) = make_float4(d[x][0] * ex2(end - G[0]), d[x][1] * ex2(end - G[1]), d[x][2] * ex2(end - G[2]), d[x][3] * ex2(end - G[3]));
+        }
+        g2[x] = __shfl_sync(0xffffffffu, up[x], 31);
     }
 }
 
@@ -116,67 +134,70 @@ struct Own {
 template <int PC> __device__ __forceinline__ void tm_ld(float (&x)[PC], uint32_t t);
 template <> __device__ __forceinline__ void tm_ld<32>(float (&x)[32], uint32_t t) { tmem_ld32(x, t); }
 template <> __device__ __forceinline__ void tm_ld<16>(float (&x)[16], uint32_t t) { tmem_ld16(x, t); }
-__device__ __forceinline__ void tm_st32f(uint32_t t, const float (&x)[32]) {
-    const uint32_t* r = reinterpret_cast<const uint32_t*>(x);
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-                 "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n"
-                 :: "r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-                    "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
-                    "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
-                    "r"(r[30]), "r"(r[31]) : "memory");
-    asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+__device__ __forceinline__ void tm_st8(uint32_t t, const uint32_t (&w)[8]) {        // (waited for by tm_wait_st)
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n"
+                 :: "r"(t), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
+__device__ __forceinline__ void tm_st16(uint32_t t, const uint32_t (&w)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n"
+                 :: "r"(t), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]),
+                    "r"(w[8]), "r"(w[9]), "r"(w[10]), "r"(w[11]), "r"(w[12]), "r"(w[13]), "r"(w[14]), "r"(w[15]) : "memory");
+}
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int32_t x, int32_t y, int32_t t, const void* src) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n"
+                 :: "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(t), "r"(smem_u32(src)) : "memory");
+}
+
+struct Maps { CUtensorMap x, B, C, z, y; };
 
 // -------------------------------------------------------------------------------------------------
 // What a block makes of an empty state.  Its products take d x e^{..} in three bf16 pieces where somebody will see the state (24 bits), in one
 // where only y will.  Every chunk's sum starts from zero and is added to the states in fp32 arithmetic.
 // -------------------------------------------------------------------------------------------------
-enum { A_W0 = 1, A_W1, A_F0, A_F1 };
-template <int NPAN>
+// A_NEXT: a chunk's tiles and steps are there, and the place of its first half is free; A_F: that of its second half is; A_W: [half][chunk
+// parity] tokens are in place; A_R: [chunk parity] the products of a chunk are issued; A_END: all of them are complete
+enum { A_NEXT = 1, A_F, A_W, A_R = A_W + 4, A_END = A_R + 2 };
 struct SmA {
     unsigned char wx[2][3][2][TILE / 2];          // [half of the tokens][piece][head]
     unsigned char B[2][2][TILE];                  // [chunk parity][panel]
+    unsigned char x[2][2][TILE];                  // [chunk parity][head]
     float w[2][2][UQ];                            // [chunk parity][head]
     float tot[4][2];
-    uint64_t bar[2], drain;
+    uint64_t bar[2], in[2], drain;
     uint32_t tslot;
 };
 
 template <int NPAN>
-__global__ void __launch_bounds__(THREADS, 1) ssm_state_umma_kernel(SsmArgs a) {
+__global__ void __launch_bounds__(THREADS, 1) ssm_state_umma_kernel(SsmArgs a, const __grid_constant__ Maps maps) {
     if (chain_wait()) return;
     extern __shared__ __align__(1024) unsigned char raw[];
-    SmA<NPAN>& s = *reinterpret_cast<SmA<NPAN>*>(raw);
+    SmA& s = *reinterpret_cast<SmA*>(raw);
     SsmUnit u;
     if (!ssm_unit(a, blockIdx.x, u) || u.outside || (u.single(a.bl) && !a.ht)) return;
     const int hpg = a.H / a.G, pairs = (hpg + 1) / 2, grp = blockIdx.y / pairs, hl = 2 * (blockIdx.y % pairs), slab = blockIdx.z * 64;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h0 = grp * hpg + hl;
     const int chunks = (int)((u.t1 - u.t0 + UQ - 1) / UQ), pieces = a.ht ? 3 : 1;
-    if (warp == CWARPS) {
+    if (warp == W_MMA) {
         if (lane == 0) {
-            mbar_init(&s.bar[0], 1); mbar_init(&s.bar[1], 1); mbar_init(&s.drain, 1);
+            mbar_init(&s.bar[0], 1); mbar_init(&s.bar[1], 1); mbar_init(&s.in[0], 1); mbar_init(&s.in[1], 1); mbar_init(&s.drain, 1);
             fence_mbar_init();
         }
         __syncwarp();
         tmem_alloc(&s.tslot, 256);
     }
     tc_fence_before();
-    nb_sync(0);
+    nb_sync<ALL>(0);
     tc_fence_after();
     const uint32_t tm = s.tslot;
 
-    if (warp == CWARPS) {
-        bool dead = false;
+    if (warp == W_MMA) {
         constexpr uint32_t id = umma_idesc(128, 128, 1, 1);
-        for (int c = 0; c < chunks; ++c)
+        for (int c = 0; c < chunks; ++c) {
 #pragma unroll 1
             for (int hf = 0; hf < 2; ++hf) {
-                if (c > 0) {                      // the tokens' half that was there before has been taken in
-                    if (lane == 0) mbar_wait(&s.bar[hf], (c - 1) & 1, dead, a.status, 53, a.poll_budget);
-                    __syncwarp();
-                    nb_arrive(A_F0 + hf);
-                }
-                nb_sync(A_W0 + hf);
+                nb_sync<CC>(A_W + 2 * hf + (c & 1));
                 if (lane == 0) {
                     tc_fence_after();
                     const uint64_t da = umma_desc_mn128(smem_u32(s.B[c & 1][0]) + hf * (TILE / 2), TILE);
@@ -190,54 +211,85 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_state_umma_kernel(SsmArgs a) {
                 }
                 __syncwarp();
             }
+            nb_arrive<HH>(A_R + (c & 1));
+        }
         if (lane == 0) {
             umma_commit(&s.drain);
             if (!mbar_drain(&s.drain, 0)) set_status(a.status, LAMPA_ERR_TIMEOUT, 53, 0);
         }
         __syncwarp();
-        nb_arrive(A_F0);
-        nb_sync(0);
+        nb_sync<ALL>(0);
         tmem_dealloc(tm, 256);
+        return;
+    }
+    if (warp == W_CTL) {
+        bool dead = false;
+        auto load = [&](int c) {                  // the second panel of a small state is its first again
+            uint64_t* bar = &s.in[c & 1];
+            const int32_t t = (int32_t)(u.t0 + (int64_t)c * UQ);
+            mbar_expect_tx(bar, 4 * TILE);
+            tma_load_3d(s.x[c & 1][0], &maps.x, slab, h0, t, bar);
+            tma_load_3d(s.x[c & 1][1], &maps.x, slab, min(h0 + 1, a.H - 1), t, bar);
+            tma_load_3d(s.B[c & 1][0], &maps.B, 0, grp, t, bar);
+            tma_load_3d(s.B[c & 1][1], &maps.B, NPAN == 2 ? 64 : 0, grp, t, bar);
+        };
+        if (lane == 0) load(0);
+        int loaded = 1;
+        for (int c = 0; c < chunks; ++c) {
+            if (c > 1) nb_sync<HH>(A_R + (c & 1));         // the products of chunk c - 2 are issued: nobody gets further ahead
+            if (lane == 0) {
+                mbar_wait(&s.in[c & 1], (c >> 1) & 1, dead, a.status, 53, a.poll_budget);
+                if (c > 0) mbar_wait(&s.bar[0], (c - 1) & 1, dead, a.status, 53, a.poll_budget);
+            }
+            __syncwarp();
+            tc_fence_before();
+            nb_sync<CS>(A_NEXT);
+            if (lane == 0) {
+                // chunk c - 1 is taken in: its buffers are free
+                if (c > 0) mbar_wait(&s.bar[1], (c - 1) & 1, dead, a.status, 53, a.poll_budget);
+                if (c + 1 < chunks && !dead) { load(c + 1); loaded = c + 2; }
+            }
+            __syncwarp();
+            tc_fence_before();
+            nb_arrive<CC>(A_F);
+        }
+        if (lane == 0) {
+            mbar_wait(&s.bar[0], (chunks - 1) & 1, dead, a.status, 53, a.poll_budget);
+            mbar_wait(&s.bar[1], (chunks - 1) & 1, dead, a.status, 53, a.poll_budget);
+        }
+        __syncwarp();
+        tc_fence_before();
+        nb_arrive<CC>(A_END);
+        if (lane == 0 && dead) {                  // copies that nobody has waited for
+            bool ok = true;
+            for (int c = max(0, loaded - 2); c < loaded; ++c) ok = mbar_drain(&s.in[c & 1], (c >> 1) & 1) && ok;
+            if (!ok) set_status(a.status, LAMPA_ERR_TIMEOUT, 53, 1);
+        }
+        __syncwarp();
+        for (int c = max(0, chunks - 2); c < chunks; ++c) nb_sync<HH>(A_R + (c & 1));
+        nb_sync<ALL>(0);
+        return;
+    }
+    if (warp == W_TAB) {
+        const Steps p = steps_of(a, h0, hl + 1 < hpg);
+        float log_dec[2] = {0.f, 0.f}, g[2];
+        for (int c = 0; c < chunks; ++c) {
+            const int64_t t = u.t0 + (int64_t)c * UQ;
+            float* const ws[2] = {s.w[c & 1][0], s.w[c & 1][1]};
+            make_tabs<false>(a, p, ws, nullptr, t, (int)min((int64_t)UQ, u.t1 - t), g);
+            if (lane < 2) s.tot[c & 3][lane] = exp2f(lane ? g[1] : g[0]);
+            log_dec[0] += g[0]; log_dec[1] += g[1];
+            nb_sync<CS>(A_NEXT);
+        }
+        if (lane < 2 && (lane == 0 || p.has[1]) && slab == 0) a.blk_dec[(int64_t)blockIdx.x * a.H + h0 + lane] = lane ? log_dec[1] : log_dec[0];
+        nb_sync<ALL>(0);
         return;
     }
 
     const int q = warp & 3, hd = warp >> 3, half = (warp >> 2) & 1;
     const Own<NPAN> own(q, half, lane);
     constexpr int PC = Own<NPAN>::PC;
-    const int h0 = grp * hpg + hl;
-    const bool step_warp = q == 0 && half == 1;   // of its head
     const bool has = hl + hd < hpg;
-    float A2 = 0.f, bias = 0.f, dt[4], log_dec = 0.f;
-    if (step_warp && has) { A2 = a.A[h0 + hd] * LOG2E; bias = a.dt_bias ? a.dt_bias[h0 + hd] : 0.f; }
-    auto tab = [&](int c) {
-        const float g = make_tab<false>(a, s.w[c & 1][hd], nullptr, dt, (int)min((int64_t)UQ, u.t1 - (u.t0 + (int64_t)c * UQ)), A2, bias);
-        if (lane == 0) s.tot[c & 3][hd] = exp2f(g);
-        log_dec += g;
-    };
-    // x of a half chunk: 16 bytes of (head, row, 8 columns), two per thread
-    uint4 xr[2][2];
-    auto load_x = [&](int c, int hf) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int i = threadIdx.x + CT * k, col = i & 7, r = 64 * hf + ((i >> 3) & 63), xh = k;
-            const int64_t t = u.t0 + (int64_t)c * UQ + r;
-            const bool ok = c < chunks && t < u.t1 && hl + xh < hpg && slab + col * 8 < a.P;
-            xr[hf][k] = ok ? __ldg(reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.x + t * a.x_tok + (h0 + xh) * a.x_head + slab + col * 8)) : make_uint4(0u, 0u, 0u, 0u);
-        }
-    };
-    auto load_B = [&](int c) {
-        const int64_t t = u.t0 + (int64_t)c * UQ;
-        load_panels<NPAN>(smem_u32(s.B[c & 1][0]), a.B, t * a.b_tok + grp * a.b_grp, a.b_tok, (int)min((int64_t)UQ, u.t1 - t), a.N, true);
-    };
-    load_B(0);
-    load_x(0, 0);
-    load_x(0, 1);
-    if (step_warp) {
-        raw_steps(a, u.t0, u.t1, h0 + hd, has, dt);
-        tab(0);
-        raw_steps(a, u.t0 + UQ, u.t1, h0 + hd, has, dt);
-    }
-    asm volatile("bar.sync 5, 512;\n" ::: "memory");           // element warps: the first steps are there
     float st[PC];
 #pragma unroll
     for (int i = 0; i < PC; ++i) st[i] = 0.f;
@@ -248,46 +300,40 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_state_umma_kernel(SsmArgs a) {
 #pragma unroll
         for (int i = 0; i < PC; ++i) st[i] = fmaf(dec, st[i], ds[i]);
     };
+    const int col = threadIdx.x & 7, r0 = (threadIdx.x >> 3) & 63;
     for (int c = 0; c < chunks; ++c) {
+        const int n = (int)min((int64_t)UQ, u.t1 - (u.t0 + (int64_t)c * UQ));
+        nb_sync<CS>(A_NEXT);
+        tc_fence_after();
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-            if (c > 0) nb_sync(A_F0 + hf);
+            if (hf) { nb_sync<CC>(A_F); tc_fence_after(); }
+            const int row = 64 * hf + r0;
+            if (n < UQ && hf == 0) {              // what follows the sequence's last token is not its own: zero
+                for (int i = threadIdx.x; i < (UQ - n) * 16; i += CT)
+                    *reinterpret_cast<uint4*>(s.B[c & 1][(i >> 3) & 1] + swz(n + (i >> 4), i & 7)) = make_uint4(0u, 0u, 0u, 0u);
+            }
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const int i = threadIdx.x + CT * k, col = i & 7, r = (i >> 3) & 63;
-                const float w = s.w[c & 1][k][64 * hf + r];
-                const uint32_t src[4] = {xr[hf][k].x, xr[hf][k].y, xr[hf][k].z, xr[hf][k].w};
-                float v[8];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float2 f = unpack_bf16x2(src[e]);
-                    v[2 * e] = f.x * w; v[2 * e + 1] = f.y * w;
-                }
+                const float w = s.w[c & 1][k][row];
+                uint4 v = *reinterpret_cast<const uint4*>(s.x[c & 1][k] + swz(row, col));
+                if (row >= n) v = make_uint4(0u, 0u, 0u, 0u);
+                const F2 w2 = f2(w), neg = f2(-1.f);
+                F2 f[4] = {mul2(unpack2(v.x), w2), mul2(unpack2(v.y), w2), mul2(unpack2(v.z), w2), mul2(unpack2(v.w), w2)};
                 for (int p = 0; p < pieces; ++p) {
-                    uint32_t o[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        o[e] = pack_bf16x2(v[2 * e], v[2 * e + 1]);
-                        const float2 f = unpack_bf16x2(o[e]);
-                        v[2 * e] -= f.x; v[2 * e + 1] -= f.y;
-                    }
-                    *reinterpret_cast<uint4*>(s.wx[hf][p][k] + swz(r, col)) = make_uint4(o[0], o[1], o[2], o[3]);
+                    const uint4 o = make_uint4(pack2(f[0]), pack2(f[1]), pack2(f[2]), pack2(f[3]));
+                    *reinterpret_cast<uint4*>(s.wx[hf][p][k] + swz(r0, col)) = o;
+                    f[0] = fma2(unpack2(o.x), neg, f[0]); f[1] = fma2(unpack2(o.y), neg, f[1]);
+                    f[2] = fma2(unpack2(o.z), neg, f[2]); f[3] = fma2(unpack2(o.w), neg, f[3]);
                 }
             }
-            load_x(c + 1, hf);
-            if (hf == 0) cp_wait();               // B of this chunk
             fence_async_smem();
             tc_fence_before();
-            nb_arrive(A_W0 + hf);
-            if (hf == 0 && step_warp && c + 1 < chunks) {      // (nobody reads the weights of chunk c - 1 any more)
-                tab(c + 1);
-                raw_steps(a, u.t0 + (int64_t)(c + 2) * UQ, u.t1, h0 + hd, has, dt);
-            }
+            nb_arrive<CC>(A_W + 2 * hf + (c & 1));
         }
-        if (c > 0) { tc_fence_after(); take_in(c - 1); }
-        if (c + 1 < chunks) load_B(c + 1);        // the products of chunk c - 1, which read this buffer, are complete
+        if (c > 0) take_in(c - 1);
     }
-    nb_sync(A_F0);
+    nb_sync<CC>(A_END);
     tc_fence_after();
     take_in(chunks - 1);
     float* const out = a.blk + ((int64_t)blockIdx.x * a.H + h0 + hd) * a.P * a.N;
@@ -295,27 +341,43 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_state_umma_kernel(SsmArgs a) {
 #pragma unroll
         for (int i = 0; i < PC; ++i)
             if (slab + own.p0 + i < a.P) out[(int64_t)(slab + own.p0 + i) * a.N + own.n] = st[i];
-    if (step_warp && has && lane == 0 && slab == 0) a.blk_dec[(int64_t)blockIdx.x * a.H + h0 + hd] = log_dec;
     tc_fence_before();
-    nb_sync(0);
+    nb_sync<ALL>(0);
 }
 
 // -------------------------------------------------------------------------------------------------
 // The output, walking through a block from the state that enters it.
 // -------------------------------------------------------------------------------------------------
-enum { C_WX = 1, C_G, C_Y, C_P, C_DS, C_PX, C_NEXT };
+enum { C_NEXT = 1, C_WX, C_G, C_Y, C_P, C_DS, C_PX, C_YF };
 template <int NPAN>
 struct SmC {
     unsigned char C[NPAN][TILE], B[2][TILE], x[2][TILE], wx[2][TILE], z[2][TILE], S[2][NPAN * TILE / 2];
     Tab tab[2][2];                                // [chunk parity][head]
     float tot[2][2];
     int bad[2][64];                               // first row of the column that is not finite, or UQ
-    uint64_t g, y, ds, px, drain;
+    int any_bad[2];
+    uint64_t in_c, in_b, in_x, in_z, g, y, ds, px, drain;
     uint32_t tslot;
 };
 
+// z sigmoid(z) of two values.  With t = e^-|z| the denominator 1 + t lies in [1, 2], where its reciprocal is a cubic and one Newton step:
+// 1 - v p(v) = T4(2v - 3) / T4(3) with the Chebyshev polynomial T4, 1 / 577 at most, squared by the step: 3e-6.  (Through the
+// special function unit, which has a quarter of the issue rate, both the exponential and the reciprocal would bound the epilogue.)
+__device__ __forceinline__ F2 silu2(F2 z) {
+    float z0, z1, t0, t1;
+    f2_get(z, z0, z1);
+    t0 = ex2(-LOG2E * fabsf(z0));
+    t1 = ex2(-LOG2E * fabsf(z1));
+    const F2 v = add2(f2(t0, t1), f2(1.f));
+    F2 p = fma2(v, f2(-128.f / 577.f), f2(768.f / 577.f));
+    p = fma2(p, v, f2(-1696.f / 577.f));
+    p = fma2(p, v, f2(1632.f / 577.f));
+    p = mul2(p, fma2(mul2(v, p), f2(-1.f), f2(2.f)));
+    return mul2(mul2(z, f2(z0 < 0.f ? t0 : 1.f, z1 < 0.f ? t1 : 1.f)), p);
+}
+
 template <int NPAN>
-__global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a) {
+__global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a, const __grid_constant__ Maps maps) {
     if (chain_wait()) return;
     extern __shared__ __align__(1024) unsigned char raw[];
     SmC<NPAN>& s = *reinterpret_cast<SmC<NPAN>*>(raw);
@@ -333,8 +395,9 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a) {
         return;
     }
     const int chunks = (int)((u.t1 - u.t0 + UQ - 1) / UQ);
-    if (warp == CWARPS) {
+    if (warp == W_MMA) {
         if (lane == 0) {
+            mbar_init(&s.in_c, 1); mbar_init(&s.in_b, 1); mbar_init(&s.in_x, 1); mbar_init(&s.in_z, 1);
             mbar_init(&s.g, 1); mbar_init(&s.y, 1); mbar_init(&s.ds, 1); mbar_init(&s.px, 1); mbar_init(&s.drain, 1);
             fence_mbar_init();
         }
@@ -342,19 +405,19 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a) {
         tmem_alloc(&s.tslot, 512);
     }
     tc_fence_before();
-    nb_sync(0);
+    nb_sync<ALL>(0);
     tc_fence_after();
     const uint32_t tm = s.tslot;
 
-    if (warp == CWARPS) {
+    if (warp == W_MMA) {
         bool dead = false;
         const uint64_t dC = umma_desc_k128(smem_u32(s.C[0])), dBk = umma_desc_k128(smem_u32(s.B[0])), dBm = umma_desc_mn128(smem_u32(s.B[0]), TILE),
                        dS = umma_desc_mn128(smem_u32(s.S[0]), NPAN * TILE / 2), dW = umma_desc_mn128(smem_u32(s.wx[0]), TILE),
                        dX0 = umma_desc_mn128(smem_u32(s.x[0])), dX1 = umma_desc_mn128(smem_u32(s.x[1]));
-        for (int c = 0; c < chunks; ++c) {
-            const bool last = c + 1 == chunks;
-            nb_sync(C_NEXT);                      // tiles and states are there
+        auto scores_and_states = [&](int c) {     // G of chunk c as soon as its tiles are there, Y when the last chunk's has been read
             if (lane == 0) {
+                mbar_wait(&s.in_c, c & 1, dead, a.status, 54, a.poll_budget);
+                mbar_wait(&s.in_b, c & 1, dead, a.status, 54, a.poll_budget);
                 tc_fence_after();
 #pragma unroll
                 for (int k = 0; k < 4 * NPAN; ++k) {
@@ -362,29 +425,50 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a) {
                     umma_f16_ss(tm + TM_G, adv(dC, at), adv(dBk, at), umma_idesc(128, 128, 0, 0), k > 0);
                 }
                 umma_commit(&s.g);
+            }
+            __syncwarp();
+            nb_sync<CC>(C_YF);
+            if (lane == 0) {
+                tc_fence_after();
 #pragma unroll
                 for (int k = 0; k < 4 * NPAN; ++k)
                     umma_f16_ss(tm + TM_Y, adv(dC, (k >> 2) * TILE + (k & 3) * 32), adv(dS, 2048 * k), umma_idesc(128, 128, 0, 1), k > 0);
                 umma_commit(&s.y);
             }
             __syncwarp();
-            nb_sync(C_WX);
+        };
+        const int h1 = min(h0 + 1, a.H - 1);
+        int asked_z = 0;
+        auto load_z = [&](int c) {
+            const int32_t t = (int32_t)(u.t0 + (int64_t)c * UQ);
+            mbar_expect_tx(&s.in_z, 2 * TILE);
+            tma_load_3d(s.z[0], &maps.z, slab, h0, t, &s.in_z);
+            tma_load_3d(s.z[1], &maps.z, slab, h1, t, &s.in_z);
+            ++asked_z;
+        };
+        if (lane == 0 && a.z_vec) load_z(0);
+        scores_and_states(0);
+        for (int c = 0; c < chunks; ++c) {
+            const bool last = c + 1 == chunks;
+            nb_sync<ALL>(C_NEXT);
+            if (lane == 0 && c > 0) {             // the last chunk's output lies in z's place; when it has been read, z may follow
+                const int32_t t = (int32_t)(u.t0 + (int64_t)(c - 1) * UQ);
+                tma_store_3d(&maps.y, slab, h0, t, s.z[0]);
+                if (hl + 1 < hpg) tma_store_3d(&maps.y, slab, h1, t, s.z[1]);
+                bulk_commit();
+                bulk_wait_read();
+                if (a.z_vec && !dead) load_z(c);
+            }
+            __syncwarp();
+            nb_sync<CC>(C_WX);
             if (lane == 0 && !last) {
                 tc_fence_after();
 #pragma unroll
-                for (int k = 0; k < 8; ++k) umma_f16_ss(tm + TM_S, adv(dBm, 2048 * k), adv(dW, 2048 * k), umma_idesc(128, 128, 1, 1), k > 0);
+                for (int k = 0; k < 8; ++k) umma_f16_ss(tm + TM_S, adv(dBm, 2048 * k), adv(dW, 2048 * k), umma_idesc(128, 128, 1, 1), 1);
                 umma_commit(&s.ds);
             }
             __syncwarp();
-            if (lane == 0) mbar_wait(&s.g, c & 1, dead, a.status, 54, a.poll_budget);
-            __syncwarp();
-            tc_fence_before();
-            nb_arrive(C_G);
-            if (lane == 0) mbar_wait(&s.y, c & 1, dead, a.status, 54, a.poll_budget);
-            __syncwarp();
-            tc_fence_before();
-            nb_arrive(C_Y);
-            nb_sync(C_P);
+            nb_sync<CC>(C_P);
             if (lane == 0) {
                 tc_fence_after();
 #pragma unroll
@@ -394,24 +478,101 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a) {
                 umma_commit(&s.px);
             }
             __syncwarp();
-            if (!last) {
-                if (lane == 0) mbar_wait(&s.ds, c & 1, dead, a.status, 54, a.poll_budget);
-                __syncwarp();
-                tc_fence_before();
-                nb_arrive(C_DS);
-            }
-            if (lane == 0) mbar_wait(&s.px, c & 1, dead, a.status, 54, a.poll_budget);
-            __syncwarp();
-            tc_fence_before();
-            nb_arrive(C_PX);
+            if (!last) scores_and_states(c + 1);
         }
         if (lane == 0) {
             umma_commit(&s.drain);
-            if (!mbar_drain(&s.drain, 0)) set_status(a.status, LAMPA_ERR_TIMEOUT, 54, 0);
+            bool ok = mbar_drain(&s.drain, 0);
+            if (asked_z) ok = mbar_drain(&s.in_z, (asked_z - 1) & 1) && ok;
+            if (!ok) set_status(a.status, LAMPA_ERR_TIMEOUT, 54, 0);
         }
         __syncwarp();
-        nb_sync(0);
+        nb_sync<ALL>(0);
         tmem_dealloc(tm, 512);
+        return;
+    }
+    if (warp == W_CTL) {
+        bool dead = false;
+        const int h1 = min(h0 + 1, a.H - 1);
+        auto tok = [&](int c) { return (int32_t)(u.t0 + (int64_t)c * UQ); };
+        auto load_C = [&](int c) {
+            mbar_expect_tx(&s.in_c, NPAN * TILE);
+#pragma unroll
+            for (int p = 0; p < NPAN; ++p) tma_load_3d(s.C[p], &maps.C, 64 * p, grp, tok(c), &s.in_c);
+        };
+        auto load_B = [&](int c) {                // the second panel of a small state is its first again
+            mbar_expect_tx(&s.in_b, 2 * TILE);
+            tma_load_3d(s.B[0], &maps.B, 0, grp, tok(c), &s.in_b);
+            tma_load_3d(s.B[1], &maps.B, NPAN == 2 ? 64 : 0, grp, tok(c), &s.in_b);
+        };
+        auto load_x = [&](int c) {
+            mbar_expect_tx(&s.in_x, 2 * TILE);
+            tma_load_3d(s.x[0], &maps.x, slab, h0, tok(c), &s.in_x);
+            tma_load_3d(s.x[1], &maps.x, slab, h1, tok(c), &s.in_x);
+        };
+        // A wait that ran out (`dead`) ends the loading; what was asked for is drained at the end.
+        int asked_c = 1, asked_b = 1, asked_x = 1;
+        if (lane == 0) { load_x(0); load_C(0); load_B(0); }
+        __syncwarp();
+        nb_arrive<CS>(C_DS);
+        auto wait = [&](uint64_t* bar, int c) { mbar_wait(bar, c & 1, dead, a.status, 54, a.poll_budget); };
+        for (int c = 0; c < chunks; ++c) {
+            const bool more = c + 1 < chunks;
+            if (lane == 0) wait(&s.in_x, c);
+            __syncwarp();
+            nb_sync<ALL>(C_NEXT);
+            if (lane == 0) wait(&s.g, c);
+            __syncwarp();
+            tc_fence_before();
+            nb_arrive<CC>(C_G);
+            if (lane == 0) {
+                if (a.z_vec) wait(&s.in_z, c);
+                wait(&s.y, c);
+                if (more && !dead) { load_C(c + 1); ++asked_c; }
+            }
+            __syncwarp();
+            tc_fence_before();
+            nb_arrive<CC>(C_Y);
+            if (more) {
+                if (lane == 0) {
+                    wait(&s.ds, c);
+                    if (!dead) { load_B(c + 1); ++asked_b; }
+                }
+                __syncwarp();
+                tc_fence_before();
+                nb_arrive<CS>(C_DS);
+            }
+            if (lane == 0) {
+                wait(&s.px, c);
+                if (more && !dead) { load_x(c + 1); ++asked_x; }
+            }
+            __syncwarp();
+            tc_fence_before();
+            nb_arrive<CC>(C_PX);
+        }
+        if (lane == 0) {
+            bool ok = mbar_drain(&s.in_c, (asked_c - 1) & 1);
+            ok = mbar_drain(&s.in_b, (asked_b - 1) & 1) && ok;
+            ok = mbar_drain(&s.in_x, (asked_x - 1) & 1) && ok;
+            if (!ok) set_status(a.status, LAMPA_ERR_TIMEOUT, 54, 1);
+        }
+        __syncwarp();
+        nb_sync<ALL>(0);
+        return;
+    }
+    if (warp == W_TAB) {
+        const Steps p = steps_of(a, h0, hl + 1 < hpg);
+        for (int c = 0; c < chunks; ++c) {
+            const int64_t t = u.t0 + (int64_t)c * UQ;
+            float* const ws[2] = {s.tab[c & 1][0].w, s.tab[c & 1][1].w};
+            float g[2];
+            make_tabs<true>(a, p, ws, s.tab[c & 1], t, (int)min((int64_t)UQ, u.t1 - t), g);
+            if (lane < 2) s.tot[c & 1][lane] = exp2f(lane ? g[1] : g[0]);
+            __syncwarp();
+            nb_arrive<CS>(C_DS);                  // the states that enter chunk c may be decayed for what it adds
+            nb_sync<ALL>(C_NEXT);
+        }
+        nb_sync<ALL>(0);
         return;
     }
 
@@ -419,259 +580,281 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a) {
     const Own<NPAN> own(q, half, lane);
     constexpr int PC = Own<NPAN>::PC;
     const int h = h0 + hd;
-    const bool has = hl + hd < hpg, step_warp = q == 0 && half == 1;
+    const bool has = hl + hd < hpg;
     const uint32_t tl = tm + ((uint32_t)(32 * q) << 16);
-    float A2 = 0.f, bias = 0.f, dt[4];
-    if (step_warp && has) { A2 = a.A[h] * LOG2E; bias = a.dt_bias ? a.dt_bias[h] : 0.f; }
-    auto tab = [&](int c) {
-        const float g = make_tab<true>(a, s.tab[c & 1][hd].w, &s.tab[c & 1][hd], dt, (int)min((int64_t)UQ, u.t1 - (u.t0 + (int64_t)c * UQ)), A2, bias);
-        if (lane == 0) s.tot[c & 1][hd] = exp2f(g);
-    };
-    auto rows_of = [&](int c) { return (int)min((int64_t)UQ, u.t1 - (u.t0 + (int64_t)c * UQ)); };
-    auto load_C = [&](int c) { load_panels<NPAN>(smem_u32(s.C[0]), a.C, (u.t0 + (int64_t)c * UQ) * a.c_tok + grp * a.c_grp, a.c_tok, rows_of(c), a.N, false); };
-    auto load_B = [&](int c) { load_panels<NPAN>(smem_u32(s.B[0]), a.B, (u.t0 + (int64_t)c * UQ) * a.b_tok + grp * a.b_grp, a.b_tok, rows_of(c), a.N, true); };
-    auto load_x = [&](int c) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-            load_panels<1>(smem_u32(s.x[k]), a.x, (u.t0 + (int64_t)c * UQ) * a.x_tok + (h0 + k) * a.x_head + slab, a.x_tok, hl + k < hpg ? rows_of(c) : 0, a.P - slab, false);
-    };
-    // this warp's part of z: 32 rows of 64 bytes
-    unsigned char* const zt = s.z[hd];
-    auto load_z = [&](int c) {
-        if (!a.z || !has) return;
-        const int n = rows_of(c);
-        const __nv_bfloat16* src = (const __nv_bfloat16*)a.z + (u.t0 + (int64_t)c * UQ) * a.z_tok + h * a.z_head + slab;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int r = 32 * q + 8 * k + (lane >> 2), c16 = 4 * half + (lane & 3);
-            const bool ok = r < n && slab + c16 * 8 < a.P;
-            if (a.z_vec) cp16(smem_u32(zt) + swz(r, c16), ok ? src + (int64_t)r * a.z_tok + c16 * 8 : src, ok);
-            else {
-                uint32_t w[4] = {0u, 0u, 0u, 0u};
-                if (ok)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) w[e >> 1] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(src + (int64_t)r * a.z_tok + c16 * 8 + e)) << (16 * (e & 1));
-                *reinterpret_cast<uint4*>(zt + swz(r, c16)) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-        }
-    };
-    load_C(0);
-    load_B(0);
-    load_x(0);
-    load_z(0);
-    if (step_warp) {
-        raw_steps(a, u.t0, u.t1, h, has, dt);
-        tab(0);
-        raw_steps(a, u.t0 + UQ, u.t1, h, has, dt);
-    }
     if (threadIdx.x < 128) s.bad[threadIdx.x >> 6][threadIdx.x & 63] = UQ;
+    if (threadIdx.x < 2) s.any_bad[threadIdx.x] = 0;
     // scores above the diagonal stay zero
-    for (int b = max(q + 1, 2 * half); b < 2 * half + 2; ++b) {
-        const uint32_t zero[16] = {};
-        tmem_st16(tl + TM_P + 64 * hd + 16 * b, zero);
+    for (int b = q + 1; b < 4; ++b) {
+        const uint32_t zero[8] = {};
+        tm_st8(tl + TM_P + 64 * hd + 16 * b + 8 * half, zero);
     }
-    const bool single = u.single(a.bl);
-    const int64_t pn = (int64_t)a.P * a.N;
-    const float* enter = !has ? nullptr : single ? (a.h0 ? a.h0 + ((int64_t)u.seq * a.H + h) * pn : nullptr) : a.blk + ((int64_t)blockIdx.x * a.H + h) * pn;
-    float st[PC];
+    tm_wait_st();
+    // 16-byte pieces of this thread's row (and state row): piece k lies at the first one's offset with k in its bits 4 and up flipped
+    const int at0 = swz(row, 4 * half), sat0 = swz(own.n, own.p0 / 8);
+    // 16 state elements: as bf16 to the operand of the chunk's Y, decayed to the accumulator of what it adds
+    auto put_state = [&](int k, const float (&v)[16], float dec) {
+        uint32_t w[16];
 #pragma unroll
-    for (int i = 0; i < PC; ++i)
-        st[i] = enter && own.n < a.N && slab + own.p0 + i < a.P ? enter[(int64_t)(slab + own.p0 + i) * a.N + own.n] : 0.f;
-    auto put_state = [&]() {
+        for (int i = 0; i < 2; ++i)
+            *reinterpret_cast<uint4*>(s.S[hd] + (sat0 ^ ((2 * k + i) << 4))) =
+                make_uint4(pack_bf16x2(v[8 * i], v[8 * i + 1]), pack_bf16x2(v[8 * i + 2], v[8 * i + 3]),
+                           pack_bf16x2(v[8 * i + 4], v[8 * i + 5]), pack_bf16x2(v[8 * i + 6], v[8 * i + 7]));
 #pragma unroll
-        for (int k = 0; k < PC / 8; ++k)
-            *reinterpret_cast<uint4*>(s.S[hd] + swz(own.n, own.p0 / 8 + k)) =
-                make_uint4(pack_bf16x2(st[8 * k], st[8 * k + 1]), pack_bf16x2(st[8 * k + 2], st[8 * k + 3]),
-                           pack_bf16x2(st[8 * k + 4], st[8 * k + 5]), pack_bf16x2(st[8 * k + 6], st[8 * k + 7]));
+        for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[i] * dec);
+        tm_st16(tl + TM_S + 64 * hd + own.p0 + 16 * k, w);
     };
-    put_state();
-    const float Dh = has && a.D ? a.D[h] : 0.f;
-    cp_wait();
+    {
+        const bool single = u.single(a.bl);
+        const int64_t pn = (int64_t)a.P * a.N;
+        const float* enter = !has ? nullptr : single ? (a.h0 ? a.h0 + ((int64_t)u.seq * a.H + h) * pn : nullptr) : a.blk + ((int64_t)blockIdx.x * a.H + h) * pn;
+        nb_sync<CS>(C_DS);
+        const float dec = s.tot[0][hd];
+#pragma unroll
+        for (int k = 0; k < PC / 16; ++k) {
+            float v[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int p = slab + own.p0 + 16 * k + i;
+                v[i] = enter && own.n < a.N && p < a.P ? enter[(int64_t)p * a.N + own.n] : 0.f;
+            }
+            put_state(k, v, dec);
+        }
+    }
+    tm_wait_st();
     fence_async_smem();
     tc_fence_before();
-    nb_sync(C_NEXT);
+    nb_arrive<CC>(C_YF);
+    const F2 Dh = f2(has && a.D ? a.D[h] : 0.f);
 
     for (int c = 0; c < chunks; ++c) {
         const bool last = c + 1 == chunks;
-        const int n = rows_of(c);
+        const int n = (int)min((int64_t)UQ, u.t1 - (u.t0 + (int64_t)c * UQ));
         const Tab& t = s.tab[c & 1][hd];
-        // ---- wx; x stays in registers for D x
-        uint32_t xr[16];
+        nb_sync<ALL>(C_NEXT);                     // x and the steps are there
+        // ---- wx
         {
-            const float w = t.w[row];
+            const F2 w2 = f2(t.w[row]);
             float odd = 0.f;
+            uint4 xr[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) xr[k] = *reinterpret_cast<const uint4*>(s.x[hd] + (at0 ^ (k << 4)));
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const uint4 v = *reinterpret_cast<const uint4*>(s.x[hd] + swz(row, 4 * half + k));
-                xr[4 * k] = v.x; xr[4 * k + 1] = v.y; xr[4 * k + 2] = v.z; xr[4 * k + 3] = v.w;
-                uint32_t o[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float2 f = unpack_bf16x2(xr[4 * k + e]);
-                    odd = fmaf(f.x, 0.f, odd); odd = fmaf(f.y, 0.f, odd);
-                    o[e] = pack_bf16x2(f.x * w, f.y * w);
-                }
-                *reinterpret_cast<uint4*>(s.wx[hd] + swz(row, 4 * half + k)) = make_uint4(o[0], o[1], o[2], o[3]);
+                const F2 f0 = unpack2(xr[k].x), f1 = unpack2(xr[k].y), f2_ = unpack2(xr[k].z), f3 = unpack2(xr[k].w);
+                float m0, m1;
+                f2_get(add2(add2(f0, f1), add2(f2_, f3)), m0, m1);
+                odd = fmaf(m0, 0.f, odd); odd = fmaf(m1, 0.f, odd);            // NaN with any that is not finite
+                *reinterpret_cast<uint4*>(s.wx[hd] + (at0 ^ (k << 4))) =
+                    make_uint4(pack2(mul2(f0, w2)), pack2(mul2(f1, w2)), pack2(mul2(f2_, w2)), pack2(mul2(f3, w2)));
             }
-            if (odd != 0.f) {                     // NaN: some element is not finite.  It may not reach the rows above through a zero score
+            if (odd != 0.f || row >= n) {
+                // Elements that are not finite may not reach the rows above through a zero score, and what follows the sequence's last
+                // token is not its own: both become zero in the tile
+#pragma unroll 1
                 for (int e = 0; e < 32; ++e) {
-                    uint16_t* p = reinterpret_cast<uint16_t*>(s.x[hd] + swz(row, 4 * half + (e >> 3))) + (e & 7);
-                    if ((*p & 0x7f80) == 0x7f80) { *p = 0; atomicMin(&s.bad[hd][32 * half + e], row); }
+                    uint16_t* p = reinterpret_cast<uint16_t*>(s.x[hd] + (at0 ^ ((e >> 3) << 4))) + (e & 7);
+                    if (row >= n) *p = 0;
+                    else if ((*p & 0x7f80) == 0x7f80) { *p = 0; atomicMin(&s.bad[hd][32 * half + e], row); s.any_bad[hd] = 1; }
                 }
             }
         }
         fence_async_smem();
-        nb_arrive(C_WX);
-        if (step_warp && !last) {
-            tab(c + 1);
-            raw_steps(a, u.t0 + (int64_t)(c + 2) * UQ, u.t1, h, has, dt);
-        }
+        nb_arrive<CC>(C_WX);
         // ---- decayed scores
-        nb_sync(C_G);
+        nb_sync<CC>(C_G);
         tc_fence_after();
         const float Gi = t.G[row];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int b = 2 * half + k;
-            if (b > q) continue;
-            float sc[32];
-            tmem_ld32(sc, tl + TM_G + 32 * b);
-            uint32_t o[16];
-            if (b < q) {
-                const float r = ex2(Gi - t.G[32 * b + 31]);
-#pragma unroll
-                for (int j = 0; j < 32; j += 4) {
-                    const float4 f = *reinterpret_cast<const float4*>(&t.cf[32 * b + j]);
-                    o[j / 2] = pack_bf16x2(sc[j] * (f.x * r), sc[j + 1] * (f.y * r));
-                    o[j / 2 + 1] = pack_bf16x2(sc[j + 2] * (f.z * r), sc[j + 3] * (f.w * r));
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 32; j += 4) {
-                    const float4 g = *reinterpret_cast<const float4*>(&t.G[32 * b + j]), d = *reinterpret_cast<const float4*>(&t.d[32 * b + j]);
-                    const float v0 = j <= lane ? sc[j] * (ex2(Gi - g.x) * d.x) : 0.f, v1 = j + 1 <= lane ? sc[j + 1] * (ex2(Gi - g.y) * d.y) : 0.f;
-                    const float v2 = j + 2 <= lane ? sc[j + 2] * (ex2(Gi - g.z) * d.z) : 0.f, v3 = j + 3 <= lane ? sc[j + 3] * (ex2(Gi - g.w) * d.w) : 0.f;
-                    o[j / 2] = pack_bf16x2(v0, v1);
-                    o[j / 2 + 1] = pack_bf16x2(v2, v3);
-                }
-            }
-            tmem_st16(tl + TM_P + 64 * hd + 16 * b, o);
-        }
-        // ---- e^{G_i} C S^T
-        nb_sync(C_Y);
-        tc_fence_after();
-        if (!last) load_C(c + 1);
         {
-            float y[32];
-            tmem_ld32(y, tl + TM_Y + 64 * hd + 32 * half);
-            const float r = ex2(Gi);
+            // Sixteen columns of every 32-block up to the diagonal; the two warps of a row share the blocks.  Below the diagonal block
+            // e^{G_i - G_j} is a row's factor to the block's end and a column's from there, both at most 1.
+            const int j0 = 16 * half;
+            float nx[16];
+            tmem_ld16_issue(nx, tl + TM_G + j0);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) y[i] *= r;
-            tm_st32f(tl + TM_Y + 64 * hd + 32 * half, y);
+            for (int b = 0; b < 4; ++b) {
+                if (b > q) break;
+                float sc[16];
+                tmem_wait_ld();
+                tmem_loaded(nx);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) sc[j] = nx[j];
+                if (b < q) tmem_ld16_issue(nx, tl + TM_G + 32 * (b + 1) + j0);
+                uint32_t o[8];
+                if (b < q) {
+                    const F2 r = f2(ex2(Gi - t.G[32 * b + 31]));
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(&t.cf[32 * b + j0 + j]);
+                        o[j / 2] = pack2(mul2(f2(sc[j], sc[j + 1]), mul2(F2{f.x}, r)));
+                        o[j / 2 + 1] = pack2(mul2(f2(sc[j + 2], sc[j + 3]), mul2(F2{f.y}, r)));
+                    }
+                } else {
+                    const int m = lane - j0;      // the last column that counts; what lies beyond is masked as bits, whatever it is
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        const float4 g = *reinterpret_cast<const float4*>(&t.G[32 * b + j0 + j]);
+                        const ulonglong2 d = *reinterpret_cast<const ulonglong2*>(&t.d[32 * b + j0 + j]);
+                        o[j / 2] = pack2(mul2(f2(sc[j], sc[j + 1]), mul2(F2{d.x}, f2(ex2(Gi - g.x), ex2(Gi - g.y)))));
+                        o[j / 2 + 1] = pack2(mul2(f2(sc[j + 2], sc[j + 3]), mul2(F2{d.y}, f2(ex2(Gi - g.z), ex2(Gi - g.w)))));
+                        o[j / 2] &= m > j ? 0xffffffffu : m == j ? 0xffffu : 0u;
+                        o[j / 2 + 1] &= m > j + 2 ? 0xffffffffu : m == j + 2 ? 0xffffu : 0u;
+                    }
+                }
+                tm_st8(tl + TM_P + 64 * hd + 16 * b + j0 / 2, o);
+            }
         }
+        // ---- e^{G_i} C S^T + D x (elements that are not finite, zero by now, make no difference: their rows become NaN)
+        nb_sync<CC>(C_Y);
+        tc_fence_after();
+        {
+            const F2 r = f2(ex2(Gi));
+            float yv[2][16];
+            tmem_ld16_issue(yv[0], tl + TM_Y + 64 * hd + 32 * half);
+            tmem_ld16_issue(yv[1], tl + TM_Y + 64 * hd + 32 * half + 16);
+            tmem_wait_ld();
+            tmem_loaded(yv[0]);
+            tmem_loaded(yv[1]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float (&y)[16] = yv[k];
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(s.x[hd] + (at0 ^ ((2 * k + v) << 4)));
+                    const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float& lo = y[8 * v + 2 * e];
+                        float& hi = y[8 * v + 2 * e + 1];
+                        f2_get(fma2(Dh, unpack2(xw[e]), mul2(f2(lo, hi), r)), lo, hi);
+                    }
+                }
+                tm_st16(tl + TM_Y + 64 * hd + 32 * half + 16 * k, reinterpret_cast<const uint32_t (&)[16]>(y));
+            }
+        }
+        tm_wait_st();
         tc_fence_before();
         fence_async_smem();                       // (zeroed elements of x)
-        nb_arrive(C_P);
+        nb_arrive<CC>(C_P);
         // ---- states
         if (!last) {
-            nb_sync(C_DS);
+            nb_sync<CS>(C_DS);
             tc_fence_after();
-            load_B(c + 1);
-            float ds[PC];
-            tm_ld<PC>(ds, tl + TM_S + 64 * hd + own.p0);
-            const float dec = s.tot[c & 1][hd];
+            const float dec = s.tot[(c + 1) & 1][hd];
+            float v[PC / 16][16];
 #pragma unroll
-            for (int i = 0; i < PC; ++i) st[i] = fmaf(dec, st[i], ds[i]);
-            put_state();
+            for (int k = 0; k < PC / 16; ++k) tmem_ld16_issue(v[k], tl + TM_S + 64 * hd + own.p0 + 16 * k);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < PC / 16; ++k) {
+                tmem_loaded(v[k]);
+                put_state(k, v[k], dec);
+            }
+            fence_async_smem();
         }
-        // ---- output
-        nb_sync(C_PX);
+        // ---- gate, while the products run
+        F2 gate[16];
+        if (a.z) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                uint32_t zw[4];
+                if (a.z_vec) {
+                    const uint4 z = *reinterpret_cast<const uint4*>(s.z[hd] + (at0 ^ (v << 4)));
+                    zw[0] = z.x; zw[1] = z.y; zw[2] = z.z; zw[3] = z.w;
+                } else {                          // rows that do not begin on 16-byte boundaries
+                    const int p = slab + 32 * half + 8 * v;
+                    const uint16_t* src = (const uint16_t*)a.z + (u.t0 + (int64_t)c * UQ + row) * a.z_tok + h * a.z_head + p;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) zw[e] = has && row < n && p < a.P ? (uint32_t)__ldg(src + 2 * e) | (uint32_t)__ldg(src + 2 * e + 1) << 16 : 0u;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) gate[4 * v + e] = silu2(unpack2(zw[e]));
+            }
+        }
+        // ---- output, into z's place
+        nb_sync<CC>(C_PX);
         tc_fence_after();
-        if (!last) load_x(c + 1);
-        unsigned char* const stage = s.wx[hd];
+        uint32_t o[16];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             float y[16];
             tmem_ld16(y, tl + TM_Y + 64 * hd + 32 * half + 16 * k);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float2 f = unpack_bf16x2(xr[8 * k + e]);
-                y[2 * e] = fmaf(Dh, f.x, y[2 * e]);
-                y[2 * e + 1] = fmaf(Dh, f.y, y[2 * e + 1]);
-            }
-            if (a.z) {
-#pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    const uint4 zr = *reinterpret_cast<const uint4*>(zt + swz(row, 4 * half + 2 * k + v));
-                    const uint32_t zw[4] = {zr.x, zr.y, zr.z, zr.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 f = unpack_bf16x2(zw[e]);
-                        y[8 * v + 2 * e] *= f.x * sigmoid_fast(f.x);
-                        y[8 * v + 2 * e + 1] *= f.y * sigmoid_fast(f.y);
-                    }
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const int4 bad = *reinterpret_cast<const int4*>(&s.bad[hd][32 * half + 16 * k + i]);
-                if (row >= bad.x) y[i] = __int_as_float(0x7fc00000);
-                if (row >= bad.y) y[i + 1] = __int_as_float(0x7fc00000);
-                if (row >= bad.z) y[i + 2] = __int_as_float(0x7fc00000);
-                if (row >= bad.w) y[i + 3] = __int_as_float(0x7fc00000);
-            }
-#pragma unroll
-            for (int v = 0; v < 2; ++v)
-                *reinterpret_cast<uint4*>(stage + swz(row, 4 * half + 2 * k + v)) =
-                    make_uint4(pack_bf16x2(y[8 * v], y[8 * v + 1]), pack_bf16x2(y[8 * v + 2], y[8 * v + 3]),
-                               pack_bf16x2(y[8 * v + 4], y[8 * v + 5]), pack_bf16x2(y[8 * v + 6], y[8 * v + 7]));
-        }
-        __syncwarp();
-        if (has) {
-            __nv_bfloat16* dst = (__nv_bfloat16*)a.y + ((u.t0 + (int64_t)c * UQ) * a.H + h) * a.P + slab;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int r = 32 * q + 8 * k + (lane >> 2), c16 = 4 * half + (lane & 3);
-                if (r < n && slab + c16 * 8 < a.P)
-                    *reinterpret_cast<uint4*>(dst + (int64_t)r * a.H * a.P + c16 * 8) = *reinterpret_cast<const uint4*>(stage + swz(r, c16));
+                F2 v = f2(y[2 * e], y[2 * e + 1]);
+                if (a.z) v = mul2(v, gate[8 * k + e]);
+                o[8 * k + e] = pack2(v);
             }
         }
-        if (last) break;
-        __syncwarp();
-        load_z(c + 1);
-        cp_wait();
-        fence_async_smem();
+        tm_wait_st();
         tc_fence_before();
-        nb_sync(C_NEXT);
+        if (!last) nb_arrive<CC>(C_YF);           // the next chunk's Y may come
+        if (s.any_bad[hd])
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+                if (row >= s.bad[hd][32 * half + e]) o[e >> 1] = (o[e >> 1] & (e & 1 ? 0xffffu : 0xffff0000u)) | (e & 1 ? 0x7fc00000u : 0x7fc0u);
+        unsigned char* const stage = s.z[hd];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) *reinterpret_cast<uint4*>(stage + (at0 ^ (v << 4))) = make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+        fence_async_smem();
+        if (!last) continue;                      // (stored by the warp that issues the products)
+        __syncwarp();
+        {                                         // rows r and r + 4 together: their pieces lie in different banks
+            const int r0 = 32 * q + ((lane >> 3) & 3) + (lane & 4), c16 = 4 * half + (lane & 3);
+            const unsigned char* src = stage + swz(r0, c16);
+            __nv_bfloat16* dst = (__nv_bfloat16*)a.y + ((u.t0 + (int64_t)c * UQ + r0) * a.H + h) * a.P + slab + c16 * 8;
+            const int left = has && slab + c16 * 8 < a.P ? n - r0 : 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (8 * k < left) *reinterpret_cast<uint4*>(dst + (int64_t)(8 * k) * a.H * a.P) = *reinterpret_cast<const uint4*>(src + 1024 * k);
+        }
     }
     tc_fence_before();
-    nb_sync(0);
+    nb_sync<ALL>(0);
+}
+
+// [n_tok][heads][cols] with the given distances (elements) as boxes of 64 columns of one head and 128 tokens; columns beyond the head's
+// read as zero
+bool make_map3(CUtensorMap* m, const void* base, int64_t n_tok, int heads, int cols, int64_t tok, int64_t head) {
+    PFN_cuTensorMapEncodeTiled enc = tensor_map_encoder();
+    if (!enc) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)heads, (cuuint64_t)n_tok};
+    const cuuint64_t strides[2] = {(cuuint64_t)(heads > 1 ? head : 8) * 2, (cuuint64_t)(n_tok > 1 ? tok : 8) * 2};     // (those of one row are not used)
+    const cuuint32_t box[3] = {64, 1, UQ}, estr[3] = {1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int NPAN>
-int launch_pan(const SsmArgs& a, int units, bool states, bool pass, cudaStream_t st) {
+int launch_pan(const SsmArgs& a, const Maps& maps, int units, bool states, cudaStream_t st) {
     static std::atomic<uint64_t> ready_s{0}, ready_o{0};
-    static_assert(sizeof(SmA<NPAN>) <= MAX_SMEM && sizeof(SmC<NPAN>) <= MAX_SMEM, "tiles fit");
+    static_assert(sizeof(SmA) <= MAX_SMEM && sizeof(SmC<NPAN>) <= MAX_SMEM, "tiles fit");
     const dim3 grid(units, (unsigned)(a.G * ((a.H / a.G + 1) / 2)), (a.P + 63) / 64);
     if (states) {
-        if (!allow_smem(ready_s, ssm_state_umma_kernel<NPAN>, (int)sizeof(SmA<NPAN>))) return LAMPA_ERR_CUDA;
-        ProfScope prof("ssm_state", st);
-        if (launch_chained(ssm_state_umma_kernel<NPAN>, grid, dim3(THREADS), sizeof(SmA<NPAN>), st, a) != cudaSuccess) return LAMPA_ERR_CUDA;
-    }
-    if (pass) {
+        if (!allow_smem(ready_s, ssm_state_umma_kernel<NPAN>, (int)sizeof(SmA))) return LAMPA_ERR_CUDA;
+        {
+            ProfScope prof("ssm_state", st);
+            if (launch_chained(ssm_state_umma_kernel<NPAN>, grid, dim3(THREADS), sizeof(SmA), st, a, maps) != cudaSuccess) return LAMPA_ERR_CUDA;
+        }
         const int rc = launch_ssm_pass(a, st);
         if (rc != LAMPA_OK) return rc;
     }
     if (!allow_smem(ready_o, ssm_out_umma_kernel<NPAN>, (int)sizeof(SmC<NPAN>))) return LAMPA_ERR_CUDA;
     ProfScope prof("ssm_out", st);
-    return launch_chained(ssm_out_umma_kernel<NPAN>, grid, dim3(THREADS), sizeof(SmC<NPAN>), st, a) == cudaSuccess ? LAMPA_OK : LAMPA_ERR_CUDA;
+    return launch_chained(ssm_out_umma_kernel<NPAN>, grid, dim3(THREADS), sizeof(SmC<NPAN>), st, a, maps) == cudaSuccess ? LAMPA_OK : LAMPA_ERR_CUDA;
 }
 
 }  // namespace
 
-int launch_ssm_scan_umma(const SsmArgs& a, int units, bool blocks, cudaStream_t st) {
+int launch_ssm_scan_umma(SsmArgs a, int units, bool blocks, cudaStream_t st) {
+    Maps maps;
+    if (!make_map3(&maps.x, a.x, a.n_tok, a.H, a.P, a.x_tok, a.x_head) || !make_map3(&maps.B, a.B, a.n_tok, a.G, a.N, a.b_tok, a.b_grp) ||
+        !make_map3(&maps.C, a.C, a.n_tok, a.G, a.N, a.c_tok, a.c_grp)) return LAMPA_ERR_CUDA;
+    maps.z = maps.x;
+    if (!make_map3(&maps.y, a.y, a.n_tok, a.H, a.P, (int64_t)a.H * a.P, a.P)) return LAMPA_ERR_CUDA;
+    a.z_vec = a.z_vec && make_map3(&maps.z, a.z, a.n_tok, a.H, a.P, a.z_tok, a.z_head);
     const bool states = blocks || a.ht;
-    return a.N <= 64 ? launch_pan<1>(a, units, states, states, st) : launch_pan<2>(a, units, states, states, st);
+    return a.N <= 64 ? launch_pan<1>(a, maps, units, states, st) : launch_pan<2>(a, maps, units, states, st);
 }
 
 }  // namespace lampa
