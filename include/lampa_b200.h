@@ -454,8 +454,8 @@ int lampa_short_conv_resume(const void* x, int64_t x_row, const void* weight, co
  *   n = delta / sqrt(mean(delta^2) + eps) * post_weight     (post_norm == 0: n = delta * post_weight)
  *   res += scale * act(gate) * n                             (scale [D], or scale_all when scale is NULL)
  *   y = res / sqrt(mean(res^2) + eps) * pre_weight           (y NULL: the update only; delta NULL: this norm only)
- * delta [rows] rows delta_row apart; gate: one row per row, or with cu_seqlens one per sequence, gate_row apart (0: the same for
- * all); gate_act 0 none, 1 sigmoid, 2 silu; weights [D] fp32 or NULL.  With cu_seqlens a row of no sequence has no gate: its res
+ * delta [rows] rows delta_row apart; gate: of delta's type or fp32, one row per row, or with cu_seqlens one per sequence, gate_row
+ * apart (0: the same for all); gate_act 0 none, 1 sigmoid, 2 silu; weights [D] fp32 or NULL.  With cu_seqlens a row of no sequence has no gate: its res
  * stays.  D at most 8192.
  */
 int lampa_block_norm(float* res, const void* delta, int64_t delta_row, int32_t delta_dtype, const void* gate, int64_t gate_row,

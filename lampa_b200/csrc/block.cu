@@ -25,34 +25,45 @@ constexpr int RUN = 16;               // tokens per thread, at least the largest
 struct ConvArgsR {
     const void* x; const void* w; const void* bias; const int64_t* cu; void* cache; void* y; int32_t* status;
     int64_t n_tok, T, x_tok;
-    int nseq, D, W, silu, w_dt, write;
+    int nseq, D, W, silu, w_dt, write, groups;
 };
 
 template <int DT> struct Bits { using T = uint16_t; };
 template <> struct Bits<LAMPA_F32> { using T = uint32_t; };
 
+// A row's channels of a thread as they lie in memory: four, or one where rows do not allow it
+template <int DT, int VEC> struct RawRow { using T = uint2; };
+template <> struct RawRow<LAMPA_F32, 4> { using T = uint4; };
+template <int DT> struct RawRow<DT, 1> { using T = typename Bits<DT>::T; };
 template <int DT, int VEC>
-__device__ __forceinline__ void load_row(const void* x, int64_t at, float (&v)[VEC]) {
-    if constexpr (VEC == 1) v[0] = Elem<DT>::ld(x, (size_t)at);
-    else unpack_vec<DT>(__ldg(reinterpret_cast<const uint4*>((const typename Elem<DT>::T*)x + at)), v);
+__device__ __forceinline__ typename RawRow<DT, VEC>::T load_raw(const void* x, int64_t at) {
+    return __ldg(reinterpret_cast<const typename RawRow<DT, VEC>::T*>((const typename Elem<DT>::T*)x + at));
+}
+template <int DT, int VEC>
+__device__ __forceinline__ void to_float(const typename RawRow<DT, VEC>::T& raw, float (&v)[VEC]) {
+    if constexpr (VEC == 1) v[0] = Elem<DT>::ld(&raw, 0);
+    else unpack4(raw, v, DT);
 }
 
-template <int DT, int VEC, int MW>    // MW: compile-time bound on the number of taps
+// 61 440 x 1 280 in bf16: 211 us with 128 threads to 160 channel groups, 16 tokens to a thread and a weight to a load.
+template <int DT, int VEC, int MW, bool EXACT>    // MW: compile-time bound on the number of taps; EXACT: it is their number, four, and weights are 16-bit
 __global__ void __launch_bounds__(128) conv_resume_kernel(ConvArgsR a) {
     if (chain_wait()) return;
+    if (a.cu && blockIdx.x == 0) check_offsets(a.cu, a.nseq, a.n_tok, a.status, 51);
     using E = typename Bits<DT>::T;
-    if (a.cu && blockIdx.x == 0 && blockIdx.y == 0) check_offsets(a.cu, a.nseq, a.n_tok, a.status, 51);
-    const int d0 = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
-    const int64_t t_begin = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * RUN;
-    if (d0 >= a.D || t_begin >= a.n_tok) return;
-    const int W = a.W;
-    float wt[MW][VEC], bs[VEC];
+    using Raw = typename RawRow<DT, VEC>::T;
+    const int64_t item = (int64_t)blockIdx.x * 128 + threadIdx.x, run = item / a.groups;
+    const int d0 = (int)(item - run * a.groups) * VEC;
+    const int64_t t_begin = run * RUN;
+    if (t_begin >= a.n_tok) return;
+    const int W = EXACT ? MW : a.W;
+    const int64_t t_end = min(t_begin + RUN, a.n_tok);
+    constexpr int AHEAD = 4;          // rows of a batch; the next batch is asked for before the first is used
+    Raw raw[2][AHEAD];
+    auto ask = [&](int buf, int64_t t0) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-        bs[j] = a.bias ? load_as_float(a.bias, d0 + j, a.w_dt) : 0.f;
-#pragma unroll
-        for (int i = 0; i < MW; ++i) wt[i][j] = i < W ? load_as_float(a.w, (size_t)(d0 + j) * W + i, a.w_dt) : 0.f;
-    }
+        for (int k = 0; k < AHEAD; ++k) raw[buf][k] = load_raw<DT, VEC>(a.x, min(t0 + k, a.n_tok - 1) * a.x_tok + d0);
+    };
     int seq;                          // sequence of the first token; nseq: behind the last one
     int64_t bos, eos;
     auto bounds = [&]() {
@@ -76,8 +87,30 @@ __global__ void __launch_bounds__(128) conv_resume_kernel(ConvArgsR a) {
         seq = (int)(t_begin / a.T);
     }
     if (!bounds() || t_begin < bos) return;
+    // tokens that look back into the cache of a sequence of an earlier run are that run's
+    const int64_t t_first = bos < t_begin ? max(t_begin, min(eos, bos + W - 1)) : t_begin;
+    ask(0, t_first);
+
+    float wt[MW][VEC], bs[VEC];
+    if constexpr (EXACT && VEC == 4) {             // a thread's weights are 4 MW neighbours
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float f[4];
+            unpack4(__ldg(reinterpret_cast<const uint2*>((const uint16_t*)a.w + (size_t)(d0 + j) * MW)), f, a.w_dt);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) wt[i][j] = f[i];
+            bs[j] = 0.f;
+        }
+        if (a.bias) unpack4(__ldg(reinterpret_cast<const uint2*>((const uint16_t*)a.bias + d0)), bs, a.w_dt);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            bs[j] = a.bias ? load_as_float(a.bias, d0 + j, a.w_dt) : 0.f;
+#pragma unroll
+            for (int i = 0; i < MW; ++i) wt[i][j] = i < W ? load_as_float(a.w, (size_t)(d0 + j) * W + i, a.w_dt) : 0.f;
+        }
+    }
     float win[MW][VEC];               // win[i]: input W - 1 - i tokens back, i < W - 1
-    const int64_t t_end = min(t_begin + RUN, a.n_tok);
     int64_t t_stop = t_end;
     // inputs before token t of this sequence; its first token opens it
     auto history = [&](int64_t t) {
@@ -86,7 +119,7 @@ __global__ void __launch_bounds__(128) conv_resume_kernel(ConvArgsR a) {
         for (int i = 0; i < MW - 1; ++i)
             if (i < W - 1) {
                 const int64_t tt = t - (W - 1) + i;
-                if (tt >= bos) load_row<DT, VEC>(a.x, tt * a.x_tok + d0, win[i]);
+                if (tt >= bos) to_float<DT, VEC>(load_raw<DT, VEC>(a.x, tt * a.x_tok + d0), win[i]);
                 else {
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) win[i][j] = slots ? Elem<DT>::ld(slots, (size_t)j * W + W + (int)(tt - bos)) : 0.f;
@@ -103,74 +136,72 @@ __global__ void __launch_bounds__(128) conv_resume_kernel(ConvArgsR a) {
                 slots[j * W + w] = tt >= 0 ? ((const E*)a.x)[(bos + tt) * a.x_tok + d0 + j] : slots[j * W + w + (int)len];
         }
     };
-    // tokens that look back into the cache of a sequence of an earlier run are that run's
-    const int64_t t_first = bos < t_begin ? max(t_begin, min(eos, bos + W - 1)) : t_begin;
     if (t_first < eos) history(t_first);
-    constexpr int AHEAD = 8;          // rows that are asked for before the first of them is used
 #pragma unroll 1
-    for (int64_t t0 = t_first; t0 < t_stop; t0 += AHEAD) {
-        float cur[AHEAD][VEC];
-        uint4 raw[VEC > 1 ? AHEAD : 1];
+    for (int64_t t1 = t_first; t1 < t_stop; t1 += 2 * AHEAD) {
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k) {
-            const int64_t at = min(t0 + k, a.n_tok - 1) * a.x_tok + d0;
-            if constexpr (VEC > 1) raw[k] = __ldg(reinterpret_cast<const uint4*>((const typename Elem<DT>::T*)a.x + at));
-            else cur[k][0] = Elem<DT>::ld(a.x, (size_t)at);
-        }
+        for (int buf = 0; buf < 2; ++buf) {
+            const int64_t t0 = t1 + buf * AHEAD;
+            if (t0 + AHEAD < t_end + W - 1) ask(buf ^ 1, t0 + AHEAD);      // (a sequence that opens in this batch may move t_stop that far)
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k) {
-            const int64_t t = t0 + k;
-            if (t >= t_stop) break;
-            if constexpr (VEC > 1) unpack_vec<DT>(raw[k], cur[k]);
-            if (t >= eos) {                                        // the next sequence that has tokens, or what lies behind the last
-                do { ++seq; } while (seq < a.nseq && a.cu && a.cu[seq + 1] <= t);
-                if (!bounds() || bos != t) return;
-                history(t);
-            }
-            float out[VEC];
+            for (int k = 0; k < AHEAD; ++k) {
+                const int64_t t = t0 + k;
+                if (t >= t_stop) break;
+                float cur[VEC];
+                to_float<DT, VEC>(raw[buf][k], cur);
+                if (t >= eos) {                                    // the next sequence that has tokens, or what lies behind the last
+                    do { ++seq; } while (seq < a.nseq && a.cu && a.cu[seq + 1] <= t);
+                    if (!bounds() || bos != t) return;
+                    history(t);
+                }
+                float out[VEC];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                float acc = bs[j];
+                for (int j = 0; j < VEC; ++j) {
+                    float acc = bs[j];
+#pragma unroll
+                    for (int i = 0; i < MW - 1; ++i)
+                        if (i < W - 1) acc = fmaf(win[i][j], wt[i][j], acc);
+#pragma unroll
+                    for (int i = 0; i < MW; ++i)
+                        if (i == W - 1) acc = fmaf(cur[j], wt[i][j], acc);
+                    out[j] = acc;
+                }
+                if (a.silu)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) out[j] *= sigmoid_fast(out[j]);
+                if (seq >= a.nseq)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) out[j] = 0.f;
+                if constexpr (VEC == 1) Elem<DT>::st(a.y, (size_t)t * a.D + d0, out[0]);
+                else store4<DT>(a.y, (size_t)t * a.D + d0, out);
 #pragma unroll
                 for (int i = 0; i < MW - 1; ++i)
-                    if (i < W - 1) acc = fmaf(win[i][j], wt[i][j], acc);
 #pragma unroll
-                for (int i = 0; i < MW; ++i)
-                    if (i == W - 1) acc = fmaf(cur[k][j], wt[i][j], acc);
-                if (a.silu) acc *= sigmoidf_(acc);
-                out[j] = seq < a.nseq ? acc : 0.f;
+                    for (int j = 0; j < VEC; ++j)
+                        if (i < W - 2) win[i][j] = win[i + 1 < MW ? i + 1 : i][j];
+                        else if (i == W - 2) win[i][j] = cur[j];
             }
-            if constexpr (VEC == 1) Elem<DT>::st(a.y, (size_t)t * a.D + d0, out[0]);
-            else store_vec<DT>(a.y, (size_t)t * a.D + d0, out);
-#pragma unroll
-            for (int i = 0; i < MW - 1; ++i)
-#pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    if (i < W - 2) win[i][j] = win[i + 1 < MW ? i + 1 : i][j];
-                    else if (i == W - 2) win[i][j] = cur[k][j];
         }
     }
 }
 
 template <int DT, int VEC>
-int launch_conv(const ConvArgsR& a, cudaStream_t st) {
-    const int groups = (a.D + VEC - 1) / VEC;
-    int bx = 1;
-    while (bx < groups && bx < 128) bx <<= 1;
-    const dim3 block(bx, 128 / bx);
-    const int64_t runs = (a.n_tok + RUN - 1) / RUN, gx = (runs + block.y - 1) / block.y;
-    if (gx > INT32_MAX) return LAMPA_ERR_UNSUPPORTED;
-    const dim3 grid((unsigned)gx, (groups + bx - 1) / bx);
-    if (grid.y > 65535) return LAMPA_ERR_UNSUPPORTED;
-    const auto kernel = a.W <= 4 ? conv_resume_kernel<DT, VEC, 4> : conv_resume_kernel<DT, VEC, 8>;
-    return launch_chained(kernel, grid, block, 0, st, a) == cudaSuccess ? LAMPA_OK : LAMPA_ERR_CUDA;
+int launch_conv(ConvArgsR a, bool vec_w, cudaStream_t st) {
+    a.groups = (a.D + VEC - 1) / VEC;
+    const int64_t runs = (a.n_tok + RUN - 1) / RUN, grid = (runs * a.groups + 127) / 128;
+    if (grid > INT32_MAX) return LAMPA_ERR_UNSUPPORTED;
+    auto kernel = conv_resume_kernel<DT, VEC, 8, false>;
+    if (a.W == 4 && vec_w && VEC == 4) kernel = conv_resume_kernel<DT, VEC, 4, true>;
+    else if (a.W <= 4) kernel = conv_resume_kernel<DT, VEC, 4, false>;
+    return launch_chained(kernel, dim3((unsigned)grid), dim3(128), 0, st, a) == cudaSuccess ? LAMPA_OK : LAMPA_ERR_CUDA;
 }
 
 // -------------------------------------------------------------------------------------------------
 // Norms around a block, on its fp32 residual stream:
 //   n = delta rsqrt(mean(delta^2) + eps) post;   v = res + scale act(gate) n;   res = v;   y = v rsqrt(mean(v^2) + eps) pre.
-// A row lies over TPR threads (lanes of a warp, or the whole CTA for wide rows) in vectors of VEC elements, VPT per thread, and stays
-// in registers between its two sums.
+// A row lies over some lanes of a warp, or over the whole CTA where it has more than 1 024 elements, in vectors of VEC elements, VPT
+// per thread, and stays in registers between its two sums.  All of a row is asked for before the first use, its gate's sequence is
+// looked up meanwhile.  61 440 x 1 024 with a CTA to a row and the types looked at load by load: 260 us.
 // -------------------------------------------------------------------------------------------------
 constexpr int NORM_THREADS = 256;
 
@@ -182,27 +213,44 @@ struct NormArgs {
     int D, nseq, delta_dt, gate_dt, y_dt, post_norm, act, lpr;
 };
 
+// VEC elements of a type (NONE: no such input) as they lie in memory, and as floats
+constexpr int NONE = -1;
+template <int VEC, int DT> struct RawV { uint32_t w[VEC == 1 || DT == NONE ? 1 : DT == LAMPA_F32 ? VEC : VEC / 2]; };
+template <int VEC, int DT>
+__device__ __forceinline__ void load_v(RawV<VEC, DT>& r, const char* p, bool ok) {
+    if constexpr (DT == NONE) return;
+    else if constexpr (VEC == 4 && DT == LAMPA_F32) {
+        const uint4 u = ok ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0u, 0u, 0u, 0u);
+        r.w[0] = u.x; r.w[1] = u.y; r.w[2] = u.z; r.w[3] = u.w;
+    } else if constexpr (VEC == 4) {
+        const uint2 u = ok ? __ldg(reinterpret_cast<const uint2*>(p)) : make_uint2(0u, 0u);
+        r.w[0] = u.x; r.w[1] = u.y;
+    } else if constexpr (DT == LAMPA_F32) r.w[0] = ok ? __ldg(reinterpret_cast<const uint32_t*>(p)) : 0u;
+    else r.w[0] = ok ? __ldg(reinterpret_cast<const uint16_t*>(p)) : (uint16_t)0;
+}
+template <int VEC, int DT>
+__device__ __forceinline__ void floats(const RawV<VEC, DT>& r, float (&x)[VEC]) {
+    if constexpr (DT == NONE) return;
+    else if constexpr (DT == LAMPA_F32) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) x[j] = __uint_as_float(r.w[j]);
+    } else if constexpr (VEC == 1) x[0] = Elem<DT>::ld(r.w, 0);
+    else {
+#pragma unroll
+        for (int q = 0; q < VEC / 2; ++q) {
+            const float2 f = DT == LAMPA_BF16 ? make_float2(__uint_as_float(r.w[q] << 16), __uint_as_float(r.w[q] & 0xffff0000u))
+                                              : __half22float2(*reinterpret_cast<const __half2*>(&r.w[q]));
+            x[2 * q] = f.x; x[2 * q + 1] = f.y;
+        }
+    }
+}
 template <int VEC>
-__device__ __forceinline__ void load_vec(const void* p, int64_t at, int dt, bool ok, float (&v)[VEC]) {
-    if constexpr (VEC == 1) {
-        v[0] = ok ? load_as_float(p, (size_t)at, dt) : 0.f;
-    } else if (!ok) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = 0.f;
-    } else if (dt == LAMPA_F32) {
-#pragma unroll
-        for (int q = 0; q < VEC / 4; ++q) {
-            const float4 f = __ldg(reinterpret_cast<const float4*>((const float*)p + at) + q);
-            v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
-        }
+__device__ __forceinline__ void load_w(const float* p, int c, bool ok, float (&v)[VEC]) {
+    if constexpr (VEC == 4) {
+        const float4 f = ok ? __ldg(reinterpret_cast<const float4*>(p + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
     } else {
-        const uint2 u = __ldg(reinterpret_cast<const uint2*>((const uint16_t*)p + at));
-        const uint32_t w[2] = {u.x, u.y};
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const float2 f = dt == LAMPA_BF16 ? unpack_bf16x2(w[q]) : __half22float2(*reinterpret_cast<const __half2*>(&w[q]));
-            v[2 * q] = f.x; v[2 * q + 1] = f.y;
-        }
+        v[0] = ok ? __ldg(p + c) : 0.f;
     }
 }
 template <int VEC>
@@ -231,67 +279,91 @@ __device__ __forceinline__ float row_sum(float v, int lpr, float (*words)[NORM_T
     return v;
 }
 
-template <int VEC, int VPT, bool WIDE>
+template <int VEC, int VPT, bool WIDE, int DD, int GD>             // types of delta and gate
 __global__ void __launch_bounds__(NORM_THREADS) block_norm_kernel(NormArgs a) {
     if (chain_wait()) return;
+    constexpr int DB = DD == NONE ? 0 : DD == LAMPA_F32 ? 4 : 2, GB = GD == NONE ? 0 : GD == LAMPA_F32 ? 4 : 2;
     __shared__ float words[2][NORM_THREADS / 32];
-    if (a.cu && blockIdx.x == 0) check_offsets(a.cu, a.nseq, a.rows, a.status, 52);
+    if (GB && a.cu && blockIdx.x == 0) check_offsets(a.cu, a.nseq, a.rows, a.status, 52);
     int turn = 0;
-    const int lpr = WIDE ? NORM_THREADS : a.lpr, rpc = NORM_THREADS / lpr;        // rows a CTA holds
-    const int l = threadIdx.x % lpr;
-    const int nvec = a.D / VEC;
+    const int lpr = WIDE ? NORM_THREADS : VPT > 1 ? 32 : a.lpr, rpc = NORM_THREADS / lpr;      // lanes to a row, rows a CTA holds
+    const int l = threadIdx.x % lpr, c0 = l * VEC, cs = lpr * VEC; // vector v of this thread begins at column c0 + v cs
     const float inv_d = 1.f / (float)a.D;
     for (int64_t base = (int64_t)blockIdx.x * rpc; base < a.rows; base += (int64_t)gridDim.x * rpc) {
         const int64_t row = base + threadIdx.x / lpr;
-        const bool in = row < a.rows;
-        int64_t grow = row;                                        // row of the gate, or -1: no sequence, no gate
-        if (a.gate && a.cu && in) {
-            int lo = 0, hi = a.nseq + 1;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (a.cu[mid] <= row) lo = mid; else hi = mid;
-            }
-            grow = lo < a.nseq && a.cu[lo] <= row && a.cu[lo + 1] > row ? lo : -1;
-        }
-        const bool add = a.delta && (!a.cu || !a.gate || grow >= 0);
-        float r[VPT][VEC], d[VPT][VEC], g[VPT][VEC];
+        const int cols = row < a.rows ? a.D - c0 : 0;              // vector v is there if v cs < cols
+        char* const pr = (char*)a.res + (row * a.D + c0) * 4;
+        const char* const pd = (const char*)a.delta + (row * a.delta_row + c0) * DB;
+        RawV<VEC, LAMPA_F32> rr[VPT];
+        RawV<VEC, DD> dd[VPT];
+        RawV<VEC, GD> gg[VPT];
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
-            const int c = (l + lpr * v) * VEC;
-            const bool ok = in && l + lpr * v < nvec;
-            load_vec<VEC>(a.res, row * a.D + c, LAMPA_F32, ok, r[v]);
-            if (a.delta) load_vec<VEC>(a.delta, row * a.delta_row + c, a.delta_dt, ok && add, d[v]);
-            if (a.gate) load_vec<VEC>(a.gate, grow * a.gate_row + c, a.gate_dt, ok && add, g[v]);
+            load_v<VEC, LAMPA_F32>(rr[v], pr + (int64_t)v * cs * 4, v * cs < cols);
+            load_v<VEC, DD>(dd[v], pd + (int64_t)v * cs * DB, v * cs < cols);
         }
-        if (a.delta) {
+        bool add = DB > 0;                                         // a row of no sequence has no gate: its residual stays
+        if (GB) {
+            int64_t grow = row;
+            if (a.cu && cols > 0) {
+                int lo = 0, hi = a.nseq + 1;
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (__ldg(a.cu + mid) <= row) lo = mid; else hi = mid;
+                }
+                grow = lo;
+                add = lo < a.nseq && __ldg(a.cu + lo) <= row && __ldg(a.cu + lo + 1) > row;
+            }
+            const char* const pg = (const char*)a.gate + (grow * a.gate_row + c0) * GB;
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) load_v<VEC, GD>(gg[v], pg + (int64_t)v * cs * GB, add && v * cs < cols);
+        }
+        if (DB) {
             float rstd = 1.f;
             if (a.post_norm) {
                 float ss = 0.f;
 #pragma unroll
-                for (int v = 0; v < VPT; ++v)
+                for (int v = 0; v < VPT; ++v) {
+                    float x[VEC];
+                    floats<VEC, DD>(dd[v], x);
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) ss = fmaf(d[v][j], d[v][j], ss);
+                    for (int j = 0; j < VEC; ++j) ss = fmaf(x[j], x[j], ss);
+                }
                 rstd = 1.f / sqrtf(row_sum<WIDE>(ss, lpr, words, turn) * inv_d + a.eps);
             }
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
-                const int c = (l + lpr * v) * VEC;
-                const bool ok = l + lpr * v < nvec;
-                float w[VEC], s[VEC];
-                if (a.post) load_vec<VEC>(a.post, c, LAMPA_F32, ok, w);
-                if (a.scale) load_vec<VEC>(a.scale, c, LAMPA_F32, ok, s);
+                const bool ok = v * cs < cols;
+                float x[VEC], w[VEC];
+                floats<VEC, DD>(dd[v], x);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    float x = d[v][j] * rstd;
-                    if (a.post) x *= w[j];
-                    if (a.gate) {
-                        const float gv = g[v][j];
-                        x *= a.act == 0 ? gv : a.act == 1 ? sigmoidf_(gv) : gv * sigmoidf_(gv);
-                    }
-                    x *= a.scale ? s[j] : a.scale1;
-                    if (add) r[v][j] += x;
+                for (int j = 0; j < VEC; ++j) x[j] *= rstd;
+                if (a.post) {
+                    load_w<VEC>(a.post, c0 + v * cs, ok, w);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) x[j] *= w[j];
                 }
-                if (ok && in && add) put_vec<VEC>(a.res, row * a.D + c, LAMPA_F32, r[v]);
+                if (GB) {
+                    float g[VEC];
+                    floats<VEC, GD>(gg[v], g);
+                    if (a.act == 1) {
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) g[j] = sigmoidf_(g[j]);
+                    } else if (a.act == 2) {
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) g[j] *= sigmoidf_(g[j]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) x[j] *= g[j];
+                }
+                if (a.scale) load_w<VEC>(a.scale, c0 + v * cs, ok, w);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) x[j] = fmaf(x[j], a.scale ? w[j] : a.scale1, __uint_as_float(rr[v].w[j]));
+                if (add) {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) rr[v].w[j] = __float_as_uint(x[j]);
+                    if (ok) put_vec<VEC>(pr + (int64_t)v * cs * 4, 0, LAMPA_F32, x);
+                }
             }
         }
         if (!a.y) continue;
@@ -299,25 +371,24 @@ __global__ void __launch_bounds__(NORM_THREADS) block_norm_kernel(NormArgs a) {
 #pragma unroll
         for (int v = 0; v < VPT; ++v)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) ss = fmaf(r[v][j], r[v][j], ss);
+            for (int j = 0; j < VEC; ++j) ss = fmaf(__uint_as_float(rr[v].w[j]), __uint_as_float(rr[v].w[j]), ss);
         const float rstd = 1.f / sqrtf(row_sum<WIDE>(ss, lpr, words, turn) * inv_d + a.eps);
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
-            const int c = (l + lpr * v) * VEC;
-            const bool ok = l + lpr * v < nvec;
+            const bool ok = v * cs < cols;
             float w[VEC], out[VEC];
-            if (a.pre) load_vec<VEC>(a.pre, c, LAMPA_F32, ok, w);
+            if (a.pre) load_w<VEC>(a.pre, c0 + v * cs, ok, w);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) out[j] = r[v][j] * rstd * (a.pre ? w[j] : 1.f);
-            if (ok && in) put_vec<VEC>(a.y, row * a.D + c, a.y_dt, out);
+            for (int j = 0; j < VEC; ++j) out[j] = __uint_as_float(rr[v].w[j]) * rstd * (a.pre ? w[j] : 1.f);
+            if (ok) put_vec<VEC>(a.y, row * a.D + c0 + v * cs, a.y_dt, out);
         }
     }
 }
 
-template <int VEC>
+template <int VEC, int DD, int GD>
 int launch_norm(NormArgs a, cudaStream_t st) {
     const int nvec = a.D / VEC;
-    const bool wide = nvec > 128;
+    const bool wide = nvec > 256;
     int lpr = 1;
     while (lpr < nvec && lpr < 32) lpr <<= 1;
     a.lpr = lpr;
@@ -325,18 +396,28 @@ int launch_norm(NormArgs a, cudaStream_t st) {
     const unsigned grid = (unsigned)std::min<int64_t>((a.rows + rpc - 1) / rpc, (int64_t)sm_count() * 16);
     void (*kernel)(NormArgs);
     if (wide) {
-        if (vpt == 1) kernel = block_norm_kernel<VEC, 1, true>;
-        else if (vpt == 2) kernel = block_norm_kernel<VEC, 2, true>;
-        else if (vpt <= 4) kernel = block_norm_kernel<VEC, 4, true>;
-        else if (vpt <= 8) kernel = block_norm_kernel<VEC, 8, true>;
-        else if (VEC == 1 && vpt <= 32) kernel = block_norm_kernel<VEC, VEC == 1 ? 32 : 8, true>;
-        else return LAMPA_ERR_UNSUPPORTED;
+        if (vpt <= 2) kernel = block_norm_kernel<VEC, 2, true, DD, GD>;
+        else if (vpt <= 8) kernel = block_norm_kernel<VEC, 8, true, DD, GD>;
+        else kernel = block_norm_kernel<VEC, VEC == 1 ? 32 : 8, true, DD, GD>;
     } else {
-        if (vpt == 1) kernel = block_norm_kernel<VEC, 1, false>;
-        else if (vpt == 2) kernel = block_norm_kernel<VEC, 2, false>;
-        else kernel = block_norm_kernel<VEC, 4, false>;
+        if (vpt == 1) kernel = block_norm_kernel<VEC, 1, false, DD, GD>;
+        else if (vpt == 2) kernel = block_norm_kernel<VEC, 2, false, DD, GD>;
+        else if (vpt <= 4) kernel = block_norm_kernel<VEC, 4, false, DD, GD>;
+        else kernel = block_norm_kernel<VEC, 8, false, DD, GD>;
     }
     return launch_chained(kernel, dim3(grid), dim3(NORM_THREADS), 0, st, a) == cudaSuccess ? LAMPA_OK : LAMPA_ERR_CUDA;
+}
+template <int VEC, int DD>
+int launch_norm_gate(const NormArgs& a, cudaStream_t st) {         // a gate is of delta's type or fp32
+    if (!a.gate) return launch_norm<VEC, DD, NONE>(a, st);
+    if (a.gate_dt == LAMPA_F32) return launch_norm<VEC, DD, LAMPA_F32>(a, st);
+    return a.gate_dt == DD ? launch_norm<VEC, DD, DD>(a, st) : LAMPA_ERR_UNSUPPORTED;
+}
+template <int VEC>
+int launch_norm_types(const NormArgs& a, cudaStream_t st) {
+    if (!a.delta) return launch_norm<VEC, NONE, NONE>(a, st);
+    if (a.delta_dt == LAMPA_BF16) return launch_norm_gate<VEC, LAMPA_BF16>(a, st);
+    return a.delta_dt == LAMPA_F16 ? launch_norm_gate<VEC, LAMPA_F16>(a, st) : launch_norm_gate<VEC, LAMPA_F32>(a, st);
 }
 
 }  // namespace
@@ -351,14 +432,15 @@ extern "C" int lampa_short_conv_resume(const void* x, int64_t x_row, const void*
     if (W < 2 || W > 8) return LAMPA_ERR_UNSUPPORTED;
     if (n_tok == 0) return LAMPA_OK;
     if (!x || !weight || !y || (write_cache && !cache) || (!cu_seqlens && n_tok % nseq)) return LAMPA_ERR_ARG;
-    const ConvArgsR a = {x, weight, bias, cu_seqlens, cache, y, status, n_tok, n_tok / nseq, x_row, nseq, D, W, silu, w_dtype, write_cache};
+    const ConvArgsR a = {x, weight, bias, cu_seqlens, cache, y, status, n_tok, n_tok / nseq, x_row, nseq, D, W, silu, w_dtype, write_cache, 0};
     cudaStream_t st = (cudaStream_t)stream;
     ProfScope prof("short_conv_resume", st);
-    const int eb = dtype_bytes(dtype), nv = 16 / eb;
-    const bool vec = D % nv == 0 && (x_row * eb) % 16 == 0 && (((uintptr_t)x | (uintptr_t)y) & 15) == 0;
-    if (dtype == LAMPA_BF16) return vec ? launch_conv<LAMPA_BF16, 8>(a, st) : launch_conv<LAMPA_BF16, 1>(a, st);
-    if (dtype == LAMPA_F16) return vec ? launch_conv<LAMPA_F16, 8>(a, st) : launch_conv<LAMPA_F16, 1>(a, st);
-    return vec ? launch_conv<LAMPA_F32, 4>(a, st) : launch_conv<LAMPA_F32, 1>(a, st);
+    const int eb = dtype_bytes(dtype);
+    const bool vec = D % 4 == 0 && x_row % 4 == 0 && (((uintptr_t)x | (uintptr_t)y) & (4 * eb - 1)) == 0;
+    const bool vec_w = w_dtype != LAMPA_F32 && (((uintptr_t)weight | (uintptr_t)bias) & 7) == 0;
+    if (dtype == LAMPA_BF16) return vec ? launch_conv<LAMPA_BF16, 4>(a, vec_w, st) : launch_conv<LAMPA_BF16, 1>(a, false, st);
+    if (dtype == LAMPA_F16) return vec ? launch_conv<LAMPA_F16, 4>(a, vec_w, st) : launch_conv<LAMPA_F16, 1>(a, false, st);
+    return vec ? launch_conv<LAMPA_F32, 4>(a, false, st) : launch_conv<LAMPA_F32, 1>(a, false, st);
 }
 
 extern "C" int lampa_block_norm(float* res, const void* delta, int64_t delta_row, int32_t delta_dtype, const void* gate, int64_t gate_row,
@@ -379,7 +461,6 @@ extern "C" int lampa_block_norm(float* res, const void* delta, int64_t delta_row
     const bool vec = D % 4 == 0 && rows_of_four(res, D, LAMPA_F32) && rows_of_four(delta, delta_row, delta_dtype) &&
                      rows_of_four(gate, gate_row, gate_dtype) && rows_of_four(y, D, y_dtype) && rows_of_four(post_weight, 0, LAMPA_F32) &&
                      rows_of_four(pre_weight, 0, LAMPA_F32) && rows_of_four(scale, 0, LAMPA_F32);
-    if (vec && D > 32 * NORM_THREADS) return LAMPA_ERR_UNSUPPORTED;
-    if (!vec && D > 32 * NORM_THREADS) return LAMPA_ERR_UNSUPPORTED;
-    return vec ? launch_norm<4>(a, st) : launch_norm<1>(a, st);
+    if (D > 32 * NORM_THREADS) return LAMPA_ERR_UNSUPPORTED;
+    return vec ? launch_norm_types<4>(a, st) : launch_norm_types<1>(a, st);
 }

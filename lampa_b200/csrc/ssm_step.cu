@@ -18,7 +18,7 @@ namespace {
 
 constexpr int THREADS = 256;
 constexpr int MAX_W = 8;
-constexpr int ROWS = 64;              // state rows whose inputs are kept at a time
+constexpr int ROWS = THREADS;         // state rows whose inputs are kept at a time
 
 struct StepArgsS {
     const void* u; const void* dt; void* cache; float* state;
@@ -34,24 +34,95 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r)); return r; }
 __device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_nctaid.x;\n" : "=r"(r)); return r; }
 
-// Convolution of channel ch of row b; MOVE: the cache moves on too
-template <int DT, bool MOVE>
-__device__ __forceinline__ float conv_channel(const StepArgsS& a, int b, int ch, int channels) {
-    const size_t at = ((size_t)b * channels + ch) * a.W;
-    const float u = Elem<DT>::ld(a.u, (size_t)(b * a.u_row + ch));
-    float acc = a.bias ? load_as_float(a.bias, ch, a.w_dt) : 0.f;
+// The inputs of a channel's convolution (the cache's last W - 1 and the new one) and its weights.  All loads of a channel come before
+// its stores; four taps of 16-bit types (T4) are one load each, and stay packed.
+template <int DT, bool T4>
+struct Channel {
+    float v[MAX_W], w[MAX_W], b;
+    __device__ __forceinline__ void load(const StepArgsS& a, int64_t row, int ch, int channels) {
+        const size_t at = ((size_t)row * channels + ch) * a.W;
+        b = a.bias ? load_as_float(a.bias, ch, a.w_dt) : 0.f;
+        const float u = Elem<DT>::ld(a.u, (size_t)(row * a.u_row + ch));
 #pragma unroll
-    for (int i = 0; i < MAX_W; ++i) {
-        if (i >= a.W) break;
-        const float v = i == a.W - 1 ? u : Elem<DT>::ld(a.cache, at + i + 1);
-        if (MOVE) Elem<DT>::st(a.cache, at + i, v);
-        acc = fmaf(v, load_as_float(a.w, (size_t)ch * a.W + i, a.w_dt), acc);
+        for (int i = 0; i < MAX_W; ++i)
+            if (i < a.W) {
+                v[i] = i == a.W - 1 ? u : Elem<DT>::ld(a.cache, at + i + 1);
+                w[i] = load_as_float(a.w, (size_t)ch * a.W + i, a.w_dt);
+            }
     }
-    return a.silu ? acc / (1.f + expf(-acc)) : acc;
-}
+    __device__ __forceinline__ float result(const StepArgsS& a) const {
+        float acc = b;
+#pragma unroll
+        for (int i = 0; i < MAX_W; ++i)
+            if (i < a.W) acc = fmaf(v[i], w[i], acc);
+        return a.silu ? acc / (1.f + expf(-acc)) : acc;
+    }
+    __device__ __forceinline__ void move(const StepArgsS& a, int64_t row, int ch, int channels) const {
+        const size_t at = ((size_t)row * channels + ch) * a.W;
+#pragma unroll
+        for (int i = 0; i < MAX_W; ++i)
+            if (i < a.W) Elem<DT>::st(a.cache, at + i, v[i]);
+    }
+};
+template <int DT>
+struct Channel<DT, true> {
+    uint2 c, k;                       // c: the cache as it was
+    uint16_t u, b;
+    // (no branch and no use of a loaded value in here, so that all loads of a thread are on their way at once)
+    __device__ __forceinline__ void load(const StepArgsS& a, int64_t row, int ch, int channels) {
+        c = reinterpret_cast<const uint2*>(a.cache)[(size_t)row * channels + ch];
+        k = __ldg(reinterpret_cast<const uint2*>(a.w) + ch);
+        b = __ldg((const uint16_t*)(a.bias ? a.bias : a.w) + ch);
+        u = __ldg((const uint16_t*)a.u + row * a.u_row + ch);
+    }
+    __device__ __forceinline__ uint2 moved() const { return make_uint2(c.x >> 16 | c.y << 16, c.y >> 16 | (uint32_t)u << 16); }
+    __device__ __forceinline__ static float2 pair(uint32_t x, bool bf) { return bf ? unpack_bf16x2(x) : __half22float2(*reinterpret_cast<const __half2*>(&x)); }
+    __device__ __forceinline__ float result(const StepArgsS& a) const {
+        const bool bf = a.w_dt == LAMPA_BF16;
+        const uint2 m = moved();
+        const float2 v0 = pair(m.x, DT == LAMPA_BF16), v1 = pair(m.y, DT == LAMPA_BF16), w0 = pair(k.x, bf), w1 = pair(k.y, bf);
+        const float acc = fmaf(v1.y, w1.y, fmaf(v1.x, w1.x, fmaf(v0.y, w0.y, fmaf(v0.x, w0.x, a.bias ? pair(b, bf).x : 0.f))));
+        return a.silu ? acc / (1.f + expf(-acc)) : acc;
+    }
+    __device__ __forceinline__ void move(const StepArgsS& a, int64_t row, int ch, int channels) const {
+        reinterpret_cast<uint2*>(a.cache)[(size_t)row * channels + ch] = moved();
+    }
+};
 
-template <int DT, int VEC, int NV>    // NV vectors of VEC state elements per lane
-__global__ void __launch_bounds__(THREADS) ssm_step_kernel(StepArgsS a) {
+// What a row's heads of one group need beside their states
+template <int DT, bool T4>
+struct StepInputs {
+    const StepArgsS& a;
+    int b, grp, total, channels;
+    // a group's B (i < N) and C channels
+    __device__ __forceinline__ int bc_channel(int i) const { return a.H * a.P + grp * a.N + (i < a.N ? i : a.G * a.N + i - a.N); }
+    __device__ __forceinline__ void put_bc(int i, const Channel<DT, T4>& k, float* sB, float* sC) const { (i < a.N ? sB[i] : sC[i - a.N]) = k.result(a); }
+    // a state row's x and what else its head has
+    struct Row { Channel<DT, T4> x; uint32_t d, z; float bias, A, D; };
+    __device__ __forceinline__ void load_x(int r, Row& k) const {
+        const int h = grp * (a.H / a.G) + r / a.P, p = r % a.P;
+        k.x.load(a, b, h * a.P + p, channels);
+        const int64_t at = b * a.dt_row + h, az = a.z ? b * a.z_row + h * a.z_head + p : 0;
+        k.d = a.dt_dt == LAMPA_F32 ? __ldg((const uint32_t*)a.dt + at) : __ldg((const uint16_t*)a.dt + at);
+        k.z = DT == LAMPA_F32 ? __ldg((const uint32_t*)(a.z ? a.z : a.u) + az) : __ldg((const uint16_t*)(a.z ? a.z : a.u) + az);
+        k.bias = __ldg((a.dt_bias ? a.dt_bias : a.A) + h);
+        k.A = __ldg(a.A + h);
+        k.D = __ldg((a.D ? a.D : a.A) + h);
+    }
+    __device__ __forceinline__ void put_x(int r, float4& to, const Row& k) const {
+        k.x.move(a, b, grp * total + r, channels);
+        const float x = k.x.result(a), z = Elem<DT>::ld(&k.z, 0);
+        float d = load_as_float(&k.d, 0, a.dt_dt) + (a.dt_bias ? k.bias : 0.f);
+        if (a.softplus) d = fmaxf(d, 0.f) + log1pf(expf(-fabsf(d)));
+        to = make_float4(d * x, expf(d * k.A), a.D ? k.D * x : 0.f, a.z ? z / (1.f + expf(-z)) : 1.f);      // d x, exp(A d), D x, gate
+    }
+};
+
+// What bounds it.  One stream: the launch and one chain of loads (4.5 us a call, among others).  64 streams, 16 heads of 64 x 128 (67 MB): 17.3 us,
+// of which the rows alone take 13.9 (4.8 TB/s with the launch); the rest is the first loads' round trip, in all CTAs at once.  18.4 with the rows' loads in
+// front of them, 26 with 102 registers (two CTAs to an SM), 21.6 with clusters of four; the rows through a ring of bulk copies: 17.7 - 29.
+template <int DT, int VEC, int NV, bool T4>    // NV vectors of VEC state elements per lane
+__global__ void __launch_bounds__(THREADS, T4 && VEC * NV == 4 ? 4 : 1) ssm_step_kernel(StepArgsS a) {
     constexpr int UNR = NV * VEC <= 4 ? 4 : 2;
     __shared__ __align__(16) float sB[256], sC[256];
     __shared__ float4 sRow[ROWS];     // d x, exp(A d), D x, gate
@@ -66,50 +137,50 @@ __global__ void __launch_bounds__(THREADS) ssm_step_kernel(StepArgsS a) {
     const int rpw = 32 / lpr, sub = lane / lpr, l = lane % lpr;
     float* const state = a.state + ((size_t)b * a.H + grp * hpg) * a.P * a.N;
 
-    float s[UNR][NV * VEC];
-    auto load_rows = [&](int base, int end) {
+    float s[UNR][NV * VEC];           // rows of a warp in flight: as soon as one is done, the one a pass further on is asked for
+    auto load_row = [&](int k, int r, int end) {
 #pragma unroll
-        for (int k = 0; k < UNR; ++k)
-#pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                const int r = base + k * rpw + sub, n = (l + lpr * v) * VEC;
-                const bool ok = r < end && n < a.N;
-                const float* p = state + (size_t)r * a.N + n;
-                if constexpr (VEC == 4) {
-                    const float4 f = ok ? *reinterpret_cast<const float4*>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    s[k][4 * v] = f.x; s[k][4 * v + 1] = f.y; s[k][4 * v + 2] = f.z; s[k][4 * v + 3] = f.w;
-                } else {
-                    s[k][v] = ok ? *p : 0.f;
-                }
+        for (int v = 0; v < NV; ++v) {
+            const int n = (l + lpr * v) * VEC;
+            const bool ok = r < end && n < a.N;
+            const float* p = state + (size_t)r * a.N + n;
+            if constexpr (VEC == 4) {
+                const float4 f = ok ? *reinterpret_cast<const float4*>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
+                s[k][4 * v] = f.x; s[k][4 * v + 1] = f.y; s[k][4 * v + 2] = f.z; s[k][4 * v + 3] = f.w;
+            } else {
+                s[k][v] = ok ? *p : 0.f;
             }
+        }
     };
     const int step = (THREADS / 32) * rpw * UNR;                   // rows of one pass of the CTA
-    const int first = r_begin + warp * rpw * UNR;
-    load_rows(first, min(r_end, r_begin + ROWS));
-
-    for (int i = threadIdx.x; i < 2 * a.N; i += THREADS) {
-        const bool c = i >= a.N;
-        const int n = c ? i - a.N : i;
-        const float v = conv_channel<DT, false>(a, b, a.H * a.P + (c ? a.G * a.N : 0) + grp * a.N + n, channels);
-        (c ? sC : sB)[n] = v;
+    const StepInputs<DT, T4> in{a, b, grp, total, channels};
+    Channel<DT, T4> bc;
+    typename StepInputs<DT, T4>::Row own;
+    const bool has_bc = threadIdx.x < 2 * a.N;
+    bc.load(a, b, in.bc_channel(min((int)threadIdx.x, 2 * a.N - 1)), channels);
+    in.load_x(min(r_begin + (int)threadIdx.x, total - 1), own);    // (ROWS is the number of threads)
+#pragma unroll
+    for (int k = 0; k < UNR; ++k) load_row(k, r_begin + (warp * UNR + k) * rpw + sub, min(r_end, r_begin + ROWS));
+    if (has_bc) in.put_bc(threadIdx.x, bc, sB, sC);
+    for (int i = threadIdx.x + THREADS; i < 2 * a.N; i += THREADS) {
+        bc.load(a, b, in.bc_channel(i), channels);
+        in.put_bc(i, bc, sB, sC);
     }
     cluster_arrive();                                              // the caches of B and C have been read
+    cluster_wait();
+    if (rank == 0)                                                 // everybody has read the caches of B and C: they move on
+        for (int i = threadIdx.x; i < 2 * a.N; i += THREADS) {
+            if (2 * a.N > THREADS) bc.load(a, b, in.bc_channel(i), channels);
+            bc.move(a, b, in.bc_channel(i), channels);
+        }
     float Bv[NV * VEC], Cv[NV * VEC];
     for (int c0 = r_begin; c0 < r_end; c0 += ROWS) {
-        const int c1 = min(r_end, c0 + ROWS);
-        __syncthreads();
-        for (int r = c0 + threadIdx.x; r < c1; r += THREADS) {
-            const int h = grp * hpg + r / a.P, p = r % a.P;
-            const float x = conv_channel<DT, true>(a, b, h * a.P + p, channels);
-            float d = load_as_float(a.dt, (size_t)(b * a.dt_row + h), a.dt_dt) + (a.dt_bias ? a.dt_bias[h] : 0.f);
-            if (a.softplus) d = fmaxf(d, 0.f) + log1pf(expf(-fabsf(d)));
-            float gate = 1.f;
-            if (a.z) {
-                const float zv = Elem<DT>::ld(a.z, (size_t)(b * a.z_row + h * a.z_head + p));
-                gate = zv / (1.f + expf(-zv));
-            }
-            sRow[r - c0] = make_float4(d * x, expf(d * a.A[h]), a.D ? a.D[h] * x : 0.f, gate);
+        const int c1 = min(r_end, c0 + ROWS), r = c0 + threadIdx.x;
+        if (c0 != r_begin) {
+            __syncthreads();
+            if (r < c1) in.load_x(r, own);
         }
+        if (r < c1) in.put_x(r, sRow[threadIdx.x], own);
         __syncthreads();
         if (c0 == r_begin) {
 #pragma unroll
@@ -121,36 +192,37 @@ __global__ void __launch_bounds__(THREADS) ssm_step_kernel(StepArgsS a) {
                     Cv[v * VEC + e] = n < a.N ? sC[n] : 0.f;
                 }
         }
-        for (int base = c0 + warp * rpw * UNR; base < c1; base += step) {
-            if (base != first) load_rows(base, c1);
+        const int base0 = c0 + warp * rpw * UNR + sub;
+        if (c0 != r_begin)
+#pragma unroll
+            for (int k = 0; k < UNR; ++k) load_row(k, base0 + k * rpw, c1);
+#pragma unroll 1
+        for (int base = base0; base - sub < c1; base += step)
 #pragma unroll
             for (int k = 0; k < UNR; ++k) {
-                const int r = base + k * rpw + sub;
+                const int r = base + k * rpw;
                 const bool ok = r < c1;
-                const float4 in = ok ? sRow[r - c0] : make_float4(0.f, 0.f, 0.f, 0.f);
+                const float4 row = ok ? sRow[r - c0] : make_float4(0.f, 0.f, 0.f, 0.f);
+                float (&x)[NV * VEC] = s[k];
                 float dot = 0.f;
 #pragma unroll
                 for (int i = 0; i < NV * VEC; ++i) {
-                    s[k][i] = fmaf(in.y, s[k][i], in.x * Bv[i]);
-                    dot = fmaf(s[k][i], Cv[i], dot);
+                    x[i] = fmaf(row.y, x[i], row.x * Bv[i]);
+                    dot = fmaf(x[i], Cv[i], dot);
                 }
 #pragma unroll
                 for (int v = 0; v < NV; ++v) {
                     const int n = (l + lpr * v) * VEC;
                     if (!ok || n >= a.N) continue;
                     float* p = state + (size_t)r * a.N + n;
-                    if constexpr (VEC == 4) *reinterpret_cast<float4*>(p) = make_float4(s[k][4 * v], s[k][4 * v + 1], s[k][4 * v + 2], s[k][4 * v + 3]);
-                    else *p = s[k][v];
+                    if constexpr (VEC == 4) *reinterpret_cast<float4*>(p) = make_float4(x[4 * v], x[4 * v + 1], x[4 * v + 2], x[4 * v + 3]);
+                    else *p = x[v];
                 }
+                load_row(k, r + step, c1);
                 for (int o = lpr >> 1; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-                if (ok && l == 0) Elem<DT>::st(a.y, (size_t)b * a.H * a.P + (size_t)grp * total + r, (dot + in.z) * in.w);
+                if (ok && l == 0) Elem<DT>::st(a.y, (size_t)b * a.H * a.P + (size_t)grp * total + r, (dot + row.z) * row.w);
             }
-        }
     }
-    cluster_wait();
-    if (rank == 0)
-        for (int i = threadIdx.x; i < 2 * a.N; i += THREADS)
-            conv_channel<DT, true>(a, b, a.H * a.P + (i >= a.N ? a.G * a.N + i - a.N : i) + grp * a.N, channels);
 }
 
 template <typename K>
@@ -168,11 +240,11 @@ int launch(K kernel, const StepArgsS& a, int cs, int ctas, cudaStream_t st) {
     return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? LAMPA_OK : LAMPA_ERR_CUDA;
 }
 
-template <int DT>
+template <int DT, bool T4>
 int launch_dt(const StepArgsS& a, int cs, int ctas, cudaStream_t st) {
-    if (a.N % 4 || ((uintptr_t)a.state & 15)) return launch(ssm_step_kernel<DT, 1, 8>, a, cs, ctas, st);
-    if (a.N <= 128) return launch(ssm_step_kernel<DT, 4, 1>, a, cs, ctas, st);
-    return launch(ssm_step_kernel<DT, 4, 2>, a, cs, ctas, st);
+    if (a.N % 4 || ((uintptr_t)a.state & 15)) return launch(ssm_step_kernel<DT, 1, 8, T4>, a, cs, ctas, st);
+    if (a.N <= 128) return launch(ssm_step_kernel<DT, 4, 1, T4>, a, cs, ctas, st);
+    return launch(ssm_step_kernel<DT, 4, 2, T4>, a, cs, ctas, st);
 }
 
 }  // namespace
@@ -200,7 +272,8 @@ extern "C" int lampa_ssm_step(const lampa_ssm_desc* d, const void* xbc, int64_t 
     cudaStream_t st = (cudaStream_t)stream;
     ProfScope prof("ssm_step", st);
     const int ctas = (int)groups * cs;
-    if (d->dtype == LAMPA_BF16) return launch_dt<LAMPA_BF16>(a, cs, ctas, st);
-    if (d->dtype == LAMPA_F16) return launch_dt<LAMPA_F16>(a, cs, ctas, st);
-    return launch_dt<LAMPA_F32>(a, cs, ctas, st);
+    const bool t4 = taps == 4 && w_dtype != LAMPA_F32 && (((uintptr_t)conv_cache | (uintptr_t)conv_weight) & 7) == 0;
+    if (d->dtype == LAMPA_BF16) return t4 ? launch_dt<LAMPA_BF16, true>(a, cs, ctas, st) : launch_dt<LAMPA_BF16, false>(a, cs, ctas, st);
+    if (d->dtype == LAMPA_F16) return t4 ? launch_dt<LAMPA_F16, true>(a, cs, ctas, st) : launch_dt<LAMPA_F16, false>(a, cs, ctas, st);
+    return launch_dt<LAMPA_F32, false>(a, cs, ctas, st);
 }

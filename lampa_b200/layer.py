@@ -311,6 +311,9 @@ def block_norm(res: torch.Tensor, delta: Optional[torch.Tensor], post_weight: Op
             gate = gate.expand(n, gate.shape[-1])
         if tuple(gate.shape) != (n, D):
             raise ValueError(f"gate must be [{n}, {D}] or [{D}]")
+        if gate.dtype not in (torch.float32, delta.dtype):
+            L.dtype_code(gate.dtype)
+            gate = gate.float()
     for t in (delta, gate):
         if t is not None:
             L.dtype_code(t.dtype)

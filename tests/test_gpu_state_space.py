@@ -307,9 +307,11 @@ def test_step_sizes(lb, dtype, B, H, P, G, N, W):
     check_step(lb, dict(step_inputs(N, B, H, P, G, N, W, dtype, z=False, pitch=3, w_dtype=F32), D=None, conv_bias=None), activation=None, softplus=False)
 
 
-def test_step_many_rows(lb):
-    """More clusters than the GPU holds at a time"""
-    check_step(lb, step_inputs(1, 700, 2, 64, 2, 64, 4, BF))
+@pytest.mark.parametrize("B,H,P,G,N,W,dtype", [(700, 2, 64, 2, 64, 4, BF), (40, 16, 64, 1, 128, 4, BF), (30, 16, 40, 1, 256, 3, FP), (160, 3, 5, 3, 20, 4, F32),
+                                               (20, 32, 128, 1, 64, 4, BF), (19, 64, 256, 1, 16, 4, BF), (150, 2, 33, 1, 7, 4, BF)])
+def test_step_many_rows(lb, B, H, P, G, N, W, dtype):
+    """More clusters than the GPU holds at a time, and rows of a CTA that take several passes"""
+    check_step(lb, step_inputs(B, B, H, P, G, N, W, dtype, pitch=1))
 
 
 def test_steps_are_the_scan(lb):
@@ -427,12 +429,12 @@ def test_conv_offsets_on_the_device_are_checked(lb):
 
 
 # ---- norms around a block ---------------------------------------------------------------------------
-def check_norm(lb, rows, D, dtype, out, seed=0, post=True, pre=True, gate="row", act=None, scale="vec", eps=1e-5, cu=None, post_norm=True, pitch=0, on_device=True):
+def check_norm(lb, rows, D, dtype, out, seed=0, post=True, pre=True, gate="row", act=None, scale="vec", eps=1e-5, cu=None, post_norm=True, pitch=0, on_device=True, g_dtype=None):
     gen = torch.Generator(device="cuda").manual_seed(seed + rows + D)
     r = lambda *s: torch.randn(*s, generator=gen, device="cuda")  # noqa: E731
     res, delta = r(rows, D), (2 * r(rows, D + pitch)).to(dtype)[:, :D]
     n = rows if cu is None else len(cu) - 1
-    g = None if gate is None else r(n, D + pitch).to(dtype)[:, :D] if gate == "row" else r(D).to(dtype)
+    g = None if gate is None else r(n, D + pitch).to(g_dtype or dtype)[:, :D] if gate == "row" else r(D).to(g_dtype or dtype)
     sc = {"vec": r(D), "num": 0.37, None: None}[scale]
     pw, qw = (1 + 0.2 * r(D) if post else None), (1 + 0.2 * r(D) if pre else None)
     full = None if g is None else g if gate == "row" else g.expand(n, D)
@@ -456,6 +458,8 @@ def test_norm_sizes(lb, dtype, rows, D):
     check_norm(lb, rows, D, dtype, F32, gate=None, scale=None, post=False, pre=False)
     check_norm(lb, rows, D, dtype, BF, gate="one", act="silu", scale="num", pitch=4)
     check_norm(lb, rows, D, dtype, None, post_norm=False, pitch=1)
+    check_norm(lb, rows, D, dtype, dtype, act="silu", g_dtype=F32)
+    check_norm(lb, rows, D, dtype, dtype, act="silu", g_dtype=FP if dtype == BF else BF)
 
 
 @pytest.mark.parametrize("D", [128, 1028, 33])
