@@ -16,16 +16,16 @@ bool dt_ok(int dt) { return dt >= LAMPA_BF16 && dt <= LAMPA_F32; }
 // -------------------------------------------------------------------------------------------------
 // y[t, d] = act(bias[d] + sum_i w[d, i] x[t - (W-1) + i, d]); what lies before a sequence's first token is its cache's last slots
 // (zero without a cache).  cache[n, d, :] becomes the last W inputs of the sequence, those before it included.
-// A thread takes VEC channels of RUN consecutive tokens with the window in registers.  The thread that has a sequence's first
+// A thread takes VEC channels of `run` consecutive tokens with the window in registers.  The thread that has a sequence's first
 // token has all tokens that look back into the cache (W - 1 at most, also where they lie in the next run) and, knowing all of x,
 // writes the cache as well: nobody else touches these slots, so one launch suffices.
 // -------------------------------------------------------------------------------------------------
-constexpr int RUN = 16;               // tokens per thread, at least the largest W - 1
+constexpr int RUN_MIN = 16;           // tokens per thread, at least the largest W - 1
 
 struct ConvArgsR {
     const void* x; const void* w; const void* bias; const int64_t* cu; void* cache; void* y; int32_t* status;
     int64_t n_tok, T, x_tok;
-    int nseq, D, W, silu, w_dt, write, groups;
+    int nseq, D, W, silu, w_dt, write, groups, run;
 };
 
 template <int DT> struct Bits { using T = uint16_t; };
@@ -45,19 +45,20 @@ __device__ __forceinline__ void to_float(const typename RawRow<DT, VEC>::T& raw,
     else unpack4(raw, v, DT);
 }
 
-// 61 440 x 1 280 in bf16: 211 us with 128 threads to 160 channel groups, 16 tokens to a thread and a weight to a load.
+// 61 440 x 1 280 in bf16 (315 MB): 87 us, 55 % of the measured bandwidth; what is left is instructions (two of the special function unit per
+// element for SiLU, 36 us of its own) and the loads in flight that 100 registers leave room for.  Eight channels to a thread: 129 us.
 template <int DT, int VEC, int MW, bool EXACT>    // MW: compile-time bound on the number of taps; EXACT: it is their number, four, and weights are 16-bit
 __global__ void __launch_bounds__(128) conv_resume_kernel(ConvArgsR a) {
     if (chain_wait()) return;
     if (a.cu && blockIdx.x == 0) check_offsets(a.cu, a.nseq, a.n_tok, a.status, 51);
     using E = typename Bits<DT>::T;
     using Raw = typename RawRow<DT, VEC>::T;
-    const int64_t item = (int64_t)blockIdx.x * 128 + threadIdx.x, run = item / a.groups;
-    const int d0 = (int)(item - run * a.groups) * VEC;
-    const int64_t t_begin = run * RUN;
+    const int64_t item = (int64_t)blockIdx.x * 128 + threadIdx.x, no = item / a.groups;
+    const int d0 = (int)(item - no * a.groups) * VEC;
+    const int64_t t_begin = no * a.run;
     if (t_begin >= a.n_tok) return;
     const int W = EXACT ? MW : a.W;
-    const int64_t t_end = min(t_begin + RUN, a.n_tok);
+    const int64_t t_end = min(t_begin + a.run, a.n_tok);
     constexpr int AHEAD = 4;          // rows of a batch; the next batch is asked for before the first is used
     Raw raw[2][AHEAD];
     auto ask = [&](int buf, int64_t t0) {
@@ -137,49 +138,56 @@ __global__ void __launch_bounds__(128) conv_resume_kernel(ConvArgsR a) {
         }
     };
     if (t_first < eos) history(t_first);
+    // output of the token whose row is `row`, and on with the window
+    auto token = [&](const Raw& row, int64_t at, bool inside) {
+        float cur[VEC], out[VEC];
+        to_float<DT, VEC>(row, cur);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            float acc = bs[j];
+#pragma unroll
+            for (int i = 0; i < MW - 1; ++i)
+                if (i < W - 1) acc = fmaf(win[i][j], wt[i][j], acc);
+#pragma unroll
+            for (int i = 0; i < MW; ++i)
+                if (i == W - 1) acc = fmaf(cur[j], wt[i][j], acc);
+            out[j] = acc;
+        }
+        if (a.silu)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) out[j] *= sigmoid_fast(out[j]);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) out[j] = inside ? out[j] : 0.f;
+        if constexpr (VEC == 1) Elem<DT>::st(a.y, (size_t)at, out[0]);
+        else store4<DT>(a.y, (size_t)at, out);
+#pragma unroll
+        for (int i = 0; i < MW - 1; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (i < W - 2) win[i][j] = win[i + 1 < MW ? i + 1 : i][j];
+                else if (i == W - 2) win[i][j] = cur[j];
+    };
 #pragma unroll 1
     for (int64_t t1 = t_first; t1 < t_stop; t1 += 2 * AHEAD) {
 #pragma unroll
         for (int buf = 0; buf < 2; ++buf) {
             const int64_t t0 = t1 + buf * AHEAD;
             if (t0 + AHEAD < t_end + W - 1) ask(buf ^ 1, t0 + AHEAD);      // (a sequence that opens in this batch may move t_stop that far)
+            if (t0 + AHEAD <= min(eos, t_stop) && seq < a.nseq) {          // a whole batch of one sequence
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) token(raw[buf][k], (t0 + k) * a.D + d0, true);
+                continue;
+            }
 #pragma unroll
             for (int k = 0; k < AHEAD; ++k) {
                 const int64_t t = t0 + k;
                 if (t >= t_stop) break;
-                float cur[VEC];
-                to_float<DT, VEC>(raw[buf][k], cur);
                 if (t >= eos) {                                    // the next sequence that has tokens, or what lies behind the last
                     do { ++seq; } while (seq < a.nseq && a.cu && a.cu[seq + 1] <= t);
                     if (!bounds() || bos != t) return;
                     history(t);
                 }
-                float out[VEC];
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    float acc = bs[j];
-#pragma unroll
-                    for (int i = 0; i < MW - 1; ++i)
-                        if (i < W - 1) acc = fmaf(win[i][j], wt[i][j], acc);
-#pragma unroll
-                    for (int i = 0; i < MW; ++i)
-                        if (i == W - 1) acc = fmaf(cur[j], wt[i][j], acc);
-                    out[j] = acc;
-                }
-                if (a.silu)
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) out[j] *= sigmoid_fast(out[j]);
-                if (seq >= a.nseq)
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) out[j] = 0.f;
-                if constexpr (VEC == 1) Elem<DT>::st(a.y, (size_t)t * a.D + d0, out[0]);
-                else store4<DT>(a.y, (size_t)t * a.D + d0, out);
-#pragma unroll
-                for (int i = 0; i < MW - 1; ++i)
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j)
-                        if (i < W - 2) win[i][j] = win[i + 1 < MW ? i + 1 : i][j];
-                        else if (i == W - 2) win[i][j] = cur[j];
+                token(raw[buf][k], t * a.D + d0, seq < a.nseq);
             }
         }
     }
@@ -188,7 +196,11 @@ __global__ void __launch_bounds__(128) conv_resume_kernel(ConvArgsR a) {
 template <int DT, int VEC>
 int launch_conv(ConvArgsR a, bool vec_w, cudaStream_t st) {
     a.groups = (a.D + VEC - 1) / VEC;
-    const int64_t runs = (a.n_tok + RUN - 1) / RUN, grid = (runs * a.groups + 127) / 128;
+    // 32 tokens where that leaves every SM a thousand threads (fewer weights and earlier rows to a token: 87 instead of 100 us for
+    // 61 440 x 1 280 in bf16, 94 with 128), else 16 (7.7 instead of 9.6 us for 6 007 x 640)
+    a.run = RUN_MIN;
+    while (a.run < 32 && a.n_tok * a.groups / (2 * a.run) >= (int64_t)sm_count() * 1024) a.run *= 2;
+    const int64_t runs = (a.n_tok + a.run - 1) / a.run, grid = (runs * a.groups + 127) / 128;
     if (grid > INT32_MAX) return LAMPA_ERR_UNSUPPORTED;
     auto kernel = conv_resume_kernel<DT, VEC, 8, false>;
     if (a.W == 4 && vec_w && VEC == 4) kernel = conv_resume_kernel<DT, VEC, 4, true>;
@@ -432,7 +444,7 @@ extern "C" int lampa_short_conv_resume(const void* x, int64_t x_row, const void*
     if (W < 2 || W > 8) return LAMPA_ERR_UNSUPPORTED;
     if (n_tok == 0) return LAMPA_OK;
     if (!x || !weight || !y || (write_cache && !cache) || (!cu_seqlens && n_tok % nseq)) return LAMPA_ERR_ARG;
-    const ConvArgsR a = {x, weight, bias, cu_seqlens, cache, y, status, n_tok, n_tok / nseq, x_row, nseq, D, W, silu, w_dtype, write_cache, 0};
+    const ConvArgsR a = {x, weight, bias, cu_seqlens, cache, y, status, n_tok, n_tok / nseq, x_row, nseq, D, W, silu, w_dtype, write_cache, 0, 0};
     cudaStream_t st = (cudaStream_t)stream;
     ProfScope prof("short_conv_resume", st);
     const int eb = dtype_bytes(dtype);

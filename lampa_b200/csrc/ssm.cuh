@@ -24,20 +24,25 @@ struct SsmArgs {
     int bl;                           // tokens per block
     int H, P, N, G, dt_dt, softplus;
     int vec, z_vec;                   // rows of x, B and C, or of z, are 16-byte aligned
+    int z_pair, y_pair;               // two neighbours of z, or y, are one aligned word
     int whole;                        // the block kernel also has the states of sequences of one block (tcgen05 form)
     int poll_budget;
 };
 
 // A block of tokens that one CTA walks through.  Packed sequences need no table: block b of sequence s has the number
 // floor(cu[s] / bl) + s + b, which rises strictly through all blocks of all sequences in order (some numbers stay unused), so
-// that a CTA finds its sequence by bisection.  What lies behind the last offset counts as one more sequence.
+// that a warp finds its sequence by looking at 32 offsets at a time (one round trip for up to 32 sequences).  What lies behind the last
+// offset counts as one more sequence.
 struct SsmUnit {
     int seq;
     int64_t bos, eos, t0, t1;         // the sequence, and this block of it
     bool outside;                     // behind the last sequence
     __device__ __forceinline__ bool single(int bl) const { return eos - bos <= bl; }
 };
-__device__ __forceinline__ bool ssm_unit(const SsmArgs& a, int u, SsmUnit& r) {
+__device__ __forceinline__ int64_t ssm_block_of(const SsmArgs& a, int64_t t) {            // t / bl, without a 64-bit division where there are fewer rows
+    return a.n_tok <= INT32_MAX ? (int64_t)((uint32_t)min(max(t, (int64_t)0), a.n_tok) / (uint32_t)a.bl) : t / a.bl;
+}
+__device__ __forceinline__ bool ssm_unit(const SsmArgs& a, int u, SsmUnit& r) {           // whole warps
     int64_t b;
     if (a.cu == nullptr) {
         r.seq = u / a.nb;
@@ -48,15 +53,17 @@ __device__ __forceinline__ bool ssm_unit(const SsmArgs& a, int u, SsmUnit& r) {
     } else {
         int lo = 0, hi = a.nseq + 1;  // largest s with floor(cu[s] / bl) + s <= u
         while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (a.cu[mid] / a.bl + mid <= u) lo = mid; else hi = mid;
+            const int step = (hi - lo + 31) / 32, at = lo + (int)(threadIdx.x & 31) * step;
+            const uint32_t below = __ballot_sync(0xffffffffu, at < hi && ssm_block_of(a, a.cu[min(at, hi - 1)]) + at <= u);
+            if (below) lo += (31 - __clz(below)) * step;           // (the first lane's holds where the offsets are in order)
+            hi = min(hi, lo + step);
         }
         r.seq = lo;
         r.outside = lo == a.nseq;
         r.bos = a.cu[lo];
         r.eos = r.outside ? a.n_tok : a.cu[lo + 1];
         if (r.bos < 0 || r.eos < r.bos || r.eos > a.n_tok) return false;      // reported by check_offsets
-        b = u - (r.bos / a.bl + lo);
+        b = u - (ssm_block_of(a, r.bos) + lo);
         if (b < 0) return false;
     }
     r.t0 = r.bos + b * a.bl;

@@ -15,8 +15,12 @@ bool built(const lampa_ssm_desc* d) {
     return (d->dtype == LAMPA_BF16 || d->dtype == LAMPA_F16) && d->N <= 256 && d->H <= 65535 && d->P <= 65535;
 }
 
-// The tcgen05 kernels take bf16 rows in pieces of 16 bytes, and their state is one operand tile.
-bool umma_shape(const lampa_ssm_desc* d) { return d->dtype == LAMPA_BF16 && d->P % 8 == 0 && d->N % 8 == 0 && d->N <= 128; }
+// The tcgen05 kernels take bf16 rows in pieces of 16 bytes, and their state is one operand tile.  Up to 128 tokens of few heads the
+// mma.sync form is one launch that ends with the state (37 tokens, 8 heads of 64 x 64: MMA37 us; tcgen05: 20.4 in three).
+bool umma_shape(const lampa_ssm_desc* d) {
+    const bool few = d->T <= 2 * SSM_Q && (int64_t)d->B * d->H * ((d->P + 63) / 64) <= 2 * sm_count();
+    return d->dtype == LAMPA_BF16 && d->P % 8 == 0 && d->N % 8 == 0 && d->N <= 128 && !few;
+}
 
 // Tokens per block.  mma.sync: enough blocks for six CTAs to an SM; tcgen05: for one CTA (of two heads) to an SM.
 int block_tokens(const lampa_ssm_desc* d, bool umma) {
@@ -80,6 +84,8 @@ extern "C" int lampa_ssm_scan(const lampa_ssm_desc* d, const void* x, int64_t x_
     a.H = d->H; a.P = d->P; a.N = d->N; a.G = d->G; a.dt_dt = d->dt_dtype; a.softplus = d->dt_softplus;
     a.vec = vec;
     a.z_vec = z && rows16(z, z_tok, z_head);
+    a.z_pair = z && d->P % 2 == 0 && (((uintptr_t)z | (uintptr_t)(z_tok * 2) | (uintptr_t)(z_head * 2)) & 3) == 0;
+    a.y_pair = d->P % 2 == 0 && ((uintptr_t)y & 3) == 0;
     a.whole = umma;
     a.poll_budget = poll_budget();
     return umma ? launch_ssm_scan_umma(a, (int)p.units, p.blocks, (cudaStream_t)stream) : launch_ssm_scan_mma(a, d->dtype, (int)p.units, p.blocks, (cudaStream_t)stream);

@@ -23,9 +23,6 @@ namespace {
 constexpr int Q = SSM_Q;
 constexpr int THREADS = 128;
 
-template <int DT> struct Raw16 { using T = __nv_bfloat16; };
-template <> struct Raw16<LAMPA_F16> { using T = __half; };
-
 __device__ __forceinline__ bool finite_(float v) { return fabsf(v) <= 3.402823466e38f; }
 
 template <int DT, int NP, int PT>
@@ -37,43 +34,49 @@ struct Sm {
     __nv_bfloat16 S[XP][PT * LN];                                      // state as the right operand of C S^T
     __nv_bfloat16 x[XP][Q * LP];
     __nv_bfloat16 wx[3][Q * LP];                                       // d x e^{G_last - G}
-    float G[Q], d[Q], w[Q];
+    float G[2][Q], d[2][Q], w[2][Q];                                   // by chunk parity
     int bad[PT];                                                       // first row of the column that is not finite, or Q
 };
 
-// rows [0, n) of a matrix of 16-bit elements into [Q][ld] tiles of XP pieces, zero beyond n rows and `cols` columns.
-// FIND: elements that are not finite become zero and leave their row in bad[].
-template <int DT, int XP, int COLS, bool FIND>
-__device__ __forceinline__ void load_tile(__nv_bfloat16* dst, int piece, int ld, const void* base, int64_t off, int64_t pitch, int n, int cols,
-                                          bool vec, int* bad) {
-    using T = typename Raw16<DT>::T;
-    const T* src = (const T*)base + off;
-    for (int i = threadIdx.x; i < Q * (COLS / 8); i += THREADS) {
-        const int r = i / (COLS / 8), c = (i % (COLS / 8)) * 8;
-        uint4 u = make_uint4(0u, 0u, 0u, 0u);
-        if (r < n && c < cols) {
-            const T* p = src + (int64_t)r * pitch + c;
-            if (vec) u = __ldg(reinterpret_cast<const uint4*>(p));     // cols is a multiple of 8 then
-            else {
-                uint16_t e[8];
+// Rows [0, n) of a matrix of 16-bit elements as COLS-wide tile pieces of 16 bytes in a thread's registers, zero beyond n rows and `cols`
+// columns: asked for a chunk ahead where that takes few registers (tiles up to 64 wide), just before use otherwise.
+template <int COLS> struct Piece { static constexpr int N = Q * (COLS / 8) / THREADS; };
+template <int DT, int COLS>
+__device__ __forceinline__ void fetch(uint4 (&u)[Piece<COLS>::N], const void* base, int64_t off, int64_t pitch, int n, int cols, bool vec) {
+    const uint16_t* src = (const uint16_t*)base + off;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) e[k] = c + k < cols ? __ldg(reinterpret_cast<const uint16_t*>(p) + k) : (uint16_t)0;
-                u = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-            }
+    for (int k = 0; k < Piece<COLS>::N; ++k) {
+        const int i = threadIdx.x + THREADS * k, r = i / (COLS / 8), c = (i % (COLS / 8)) * 8;
+        u[k] = make_uint4(0u, 0u, 0u, 0u);
+        if (r >= n || c >= cols) continue;
+        const uint16_t* p = src + (int64_t)r * pitch + c;
+        if (vec) u[k] = __ldg(reinterpret_cast<const uint4*>(p));      // cols is a multiple of 8 then
+        else {
+            uint32_t e[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e[j] = c + j < cols ? __ldg(p + j) : (uint16_t)0;
+            u[k] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
         }
-        uint32_t w[4] = {u.x, u.y, u.z, u.w}, lo[4];
+    }
+}
+// ... into XP bf16 pieces.  FIND: elements that are not finite become zero and leave their row in bad[].
+template <int DT, int XP, int COLS, bool FIND>
+__device__ __forceinline__ void put(__nv_bfloat16* dst, int piece, int ld, const uint4 (&u)[Piece<COLS>::N], int* bad) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            float2 f = DT == LAMPA_F16 ? __half22float2(*reinterpret_cast<__half2*>(&w[k])) : unpack_bf16x2(w[k]);
+    for (int k = 0; k < Piece<COLS>::N; ++k) {
+        const int i = threadIdx.x + THREADS * k, r = i / (COLS / 8), c = (i % (COLS / 8)) * 8;
+        uint32_t w[4] = {u[k].x, u[k].y, u[k].z, u[k].w}, lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float2 f = DT == LAMPA_F16 ? __half22float2(*reinterpret_cast<__half2*>(&w[j])) : unpack_bf16x2(w[j]);
             if (FIND) {
-                const bool f0 = finite_(f.x), f1 = finite_(f.y);
-                if (!f0) { atomicMin(&bad[c + 2 * k], r); f.x = 0.f; }
-                if (!f1) { atomicMin(&bad[c + 2 * k + 1], r); f.y = 0.f; }
+                if (!finite_(f.x)) { atomicMin(&bad[c + 2 * j], r); f.x = 0.f; }
+                if (!finite_(f.y)) { atomicMin(&bad[c + 2 * j + 1], r); f.y = 0.f; }
             }
-            w[k] = pack_bf16x2(f.x, f.y);
+            w[j] = pack_bf16x2(f.x, f.y);
             if (XP > 1) {
-                const float2 h = unpack_bf16x2(w[k]);
-                lo[k] = pack_bf16x2(f.x - h.x, f.y - h.y);
+                const float2 h = unpack_bf16x2(w[j]);
+                lo[j] = pack_bf16x2(f.x - h.x, f.y - h.y);
             }
         }
         *reinterpret_cast<uint4*>(dst + r * ld + c) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -81,20 +84,24 @@ __device__ __forceinline__ void load_tile(__nv_bfloat16* dst, int piece, int ld,
     }
 }
 
-// d, G and w = d e^{G_last - G} of a chunk's n tokens (tokens beyond them have d = 0).  Returns G_last.  The first warp computes,
-// everybody else comes in behind the caller's barrier.  The exponent of w is summed from the end of the chunk: it then carries an
-// error of its own size, not of G's.
+// d, G and w = d e^{G_last - G} of a chunk's n tokens (tokens beyond them have d = 0), by the first warp, two tokens to a lane: raw steps a
+// chunk ahead, the rest while the other warps, which have more scores to work on, are busy.  The exponent of w is summed from the end of
+// the chunk: it then carries an error of its own size, not of G's.
+__device__ __forceinline__ void raw_steps(const SsmArgs& a, int64_t t0, int n, int h, float (&raw)[2]) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int i = 2 * (threadIdx.x & 31) + k;
+        raw[k] = i < n ? load_as_float(a.dt, (size_t)((t0 + i) * a.dt_tok + h), a.dt_dt) : 0.f;
+    }
+}
 template <typename SM>
-__device__ __forceinline__ void chunk_steps(const SsmArgs& a, SM& s, int64_t t0, int n, int h) {
-    if (threadIdx.x >= 32) return;
-    const int l = threadIdx.x;
-    const float A = a.A[h], bias = a.dt_bias ? a.dt_bias[h] : 0.f;
+__device__ __forceinline__ void chunk_steps(const SsmArgs& a, SM& s, int buf, const float (&raw)[2], int n, float A, float bias) {
+    const int l = threadIdx.x & 31;
     float d[2], g[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        const int i = 2 * l + k;
-        d[k] = i < n ? ssm_step_size(load_as_float(a.dt, (size_t)((t0 + i) * a.dt_tok + h), a.dt_dt) + bias, a.softplus) : 0.f;
-        g[k] = i < n ? d[k] * A : 0.f;
+        d[k] = 2 * l + k < n ? ssm_step_size(raw[k] + bias, a.softplus) : 0.f;
+        g[k] = 2 * l + k < n ? d[k] * A : 0.f;
     }
     float up = g[0] + g[1], down = up;
 #pragma unroll
@@ -105,15 +112,15 @@ __device__ __forceinline__ void chunk_steps(const SsmArgs& a, SM& s, int64_t t0,
     }
     const float before = __shfl_up_sync(0xffffffffu, up, 1), after = __shfl_down_sync(0xffffffffu, down, 1);
     const float b = l ? before : 0.f, e = l < 31 ? after : 0.f;
-    s.d[2 * l] = d[0]; s.d[2 * l + 1] = d[1];
-    s.G[2 * l] = b + g[0]; s.G[2 * l + 1] = up;
-    s.w[2 * l] = d[0] * expf(e + g[1]);
-    s.w[2 * l + 1] = d[1] * expf(e);
+    s.d[buf][2 * l] = d[0]; s.d[buf][2 * l + 1] = d[1];
+    s.G[buf][2 * l] = b + g[0]; s.G[buf][2 * l + 1] = up;
+    s.w[buf][2 * l] = d[0] * expf(e + g[1]);
+    s.w[buf][2 * l + 1] = d[1] * expf(e);
 }
 
 // wx pieces from the x tile: `pieces` of three
 template <int DT, int NP, int PT>
-__device__ __forceinline__ void scale_x(Sm<DT, NP, PT>& s, int pieces) {
+__device__ __forceinline__ void scale_x(Sm<DT, NP, PT>& s, int buf, int pieces) {
     using S = Sm<DT, NP, PT>;
     for (int i = threadIdx.x; i < Q * (PT / 2); i += THREADS) {
         const int r = i / (PT / 2), c = (i % (PT / 2)) * 2, at = r * S::LP + c;
@@ -122,7 +129,7 @@ __device__ __forceinline__ void scale_x(Sm<DT, NP, PT>& s, int pieces) {
             const float2 lo = unpack_bf16x2(*reinterpret_cast<const uint32_t*>(&s.x[S::XP - 1][at]));
             v.x += lo.x; v.y += lo.y;
         }
-        v.x *= s.w[r]; v.y *= s.w[r];
+        v.x *= s.w[buf][r]; v.y *= s.w[buf][r];
         for (int p = 0; p < pieces; ++p) {
             const uint32_t u = pack_bf16x2(v.x, v.y);
             *reinterpret_cast<uint32_t*>(&s.wx[p][at]) = u;
@@ -190,23 +197,44 @@ __device__ __forceinline__ void each_state(float (&st)[StateMap<NP, PT>::CT][2][
 template <int DT, int NP, int PT>
 __global__ void __launch_bounds__(THREADS) ssm_state_kernel(SsmArgs a) {
     if (chain_wait()) return;
-    extern __shared__ __align__(16) char raw[];
-    Sm<DT, NP, PT>& s = *reinterpret_cast<Sm<DT, NP, PT>*>(raw);
+    extern __shared__ __align__(16) char smem[];
+    Sm<DT, NP, PT>& s = *reinterpret_cast<Sm<DT, NP, PT>*>(smem);
     SsmUnit u;
     const int h = blockIdx.y, p0 = blockIdx.z * PT;
     if (!ssm_unit(a, blockIdx.x, u) || u.outside || u.single(a.bl)) return;
+    using SMT = Sm<DT, NP, PT>;
+    constexpr bool AHEAD = NP <= 64;
+    const int grp = h / (a.H / a.G);
+    const float A = a.A[h], bias = a.dt_bias ? a.dt_bias[h] : 0.f;
     float st[StateMap<NP, PT>::CT][2][4] = {};
-    float log_dec = 0.f;
-    for (int64_t t = u.t0; t < u.t1; t += Q) {
-        const int n = (int)min((int64_t)Q, u.t1 - t);
+    float log_dec = 0.f, raw[2];
+    uint4 ub[Piece<NP>::N], ux[Piece<PT>::N];
+    auto tokens = [&](int64_t t) { return (int)max((int64_t)0, min((int64_t)Q, u.t1 - t)); };
+    auto ask = [&](int64_t t) {
+        fetch<DT, NP>(ub, a.B, t * a.b_tok + grp * a.b_grp, a.b_tok, tokens(t), a.N, a.vec);
+        fetch<DT, PT>(ux, a.x, t * a.x_tok + h * a.x_head + p0, a.x_tok, tokens(t), a.P - p0, a.vec);
+    };
+    if (threadIdx.x < 32) raw_steps(a, u.t0, tokens(u.t0), h, raw);
+    if (AHEAD) ask(u.t0);
+    if (threadIdx.x < 32) {
+        chunk_steps(a, s, 0, raw, tokens(u.t0), A, bias);
+        raw_steps(a, u.t0 + Q, tokens(u.t0 + Q), h, raw);
+    }
+    int buf = 0;
+    for (int64_t t = u.t0; t < u.t1; t += Q, buf ^= 1) {
+        if (!AHEAD) ask(t);
         __syncthreads();
-        chunk_steps(a, s, t, n, h);
-        load_tile<DT, Sm<DT, NP, PT>::XP, NP, false>(s.B[0], Q * Sm<DT, NP, PT>::LN, Sm<DT, NP, PT>::LN, a.B, t * a.b_tok + (h / (a.H / a.G)) * a.b_grp, a.b_tok, n, a.N, a.vec, nullptr);
-        load_tile<DT, Sm<DT, NP, PT>::XP, PT, false>(s.x[0], Q * Sm<DT, NP, PT>::LP, Sm<DT, NP, PT>::LP, a.x, t * a.x_tok + h * a.x_head + p0, a.x_tok, n, a.P - p0, a.vec, nullptr);
+        put<DT, SMT::XP, NP, false>(s.B[0], Q * SMT::LN, SMT::LN, ub, nullptr);
+        put<DT, SMT::XP, PT, false>(s.x[0], Q * SMT::LP, SMT::LP, ux, nullptr);
         __syncthreads();
-        scale_x(s, 3);
+        if (AHEAD) ask(t + Q);
+        scale_x(s, buf, 3);
+        if (threadIdx.x < 32) {
+            chunk_steps(a, s, buf ^ 1, raw, tokens(t + Q), A, bias);
+            raw_steps(a, t + 2 * Q, tokens(t + 2 * Q), h, raw);
+        }
         __syncthreads();
-        const float g = s.G[Q - 1];
+        const float g = s.G[buf][Q - 1];
         update_state(st, s, expf(g), 3);
         log_dec += g * 1.4426950408889634f;
     }
@@ -227,7 +255,7 @@ __global__ void __launch_bounds__(256) ssm_pass_kernel(SsmArgs a) {
     if (a.cu) {
         bos = a.cu[seq]; eos = a.cu[seq + 1];
         if (bos < 0 || eos < bos || eos > a.n_tok) return;         // reported by the output kernel
-        u0 = bos / a.bl + seq;
+        u0 = ssm_block_of(a, bos) + seq;
     }
     if (e >= pn) return;
     const int64_t len = eos - bos, out = ((int64_t)seq * a.H + h) * pn + e;
@@ -255,16 +283,13 @@ __global__ void __launch_bounds__(256) ssm_pass_kernel(SsmArgs a) {
     if (a.ht) a.ht[out] = s;
 }
 
-template <int DT>
-__device__ __forceinline__ float load16(const void* p, int64_t i) { return Elem<DT>::ld(p, (size_t)i); }
-
 template <int DT, int NP, int PT>
 __global__ void __launch_bounds__(THREADS) ssm_out_kernel(SsmArgs a) {
     using SMT = Sm<DT, NP, PT>;
     constexpr int XP = SMT::XP, LN = SMT::LN, LP = SMT::LP;
     if (chain_wait()) return;
-    extern __shared__ __align__(16) char raw[];
-    SMT& s = *reinterpret_cast<SMT*>(raw);
+    extern __shared__ __align__(16) char smem[];
+    SMT& s = *reinterpret_cast<SMT*>(smem);
     SsmUnit u;
     const int h = blockIdx.y, p0 = blockIdx.z * PT, grp = h / (a.H / a.G);
     if (a.cu && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) check_offsets(a.cu, a.nseq, a.n_tok, a.status, 50);
@@ -281,30 +306,61 @@ __global__ void __launch_bounds__(THREADS) ssm_out_kernel(SsmArgs a) {
     const int pieces = single && a.ht ? 3 : XP;
     const int64_t pn = (int64_t)a.P * a.N;
     const float* enter = single ? (a.h0 ? a.h0 + ((int64_t)u.seq * a.H + h) * pn : nullptr) : a.blk + ((int64_t)blockIdx.x * a.H + h) * pn;
+    constexpr bool AHEAD = NP <= 64;
+    const float Dh = a.D ? a.D[h] : 0.f, A = a.A[h], bias = a.dt_bias ? a.dt_bias[h] : 0.f;
+    for (int i = threadIdx.x; i < PT; i += THREADS) s.bad[i] = Q;
+    float raw[2];
+    uint4 ub[Piece<NP>::N], uc[Piece<NP>::N], ux[Piece<PT>::N];
+    auto tokens = [&](int64_t t) { return (int)max((int64_t)0, min((int64_t)Q, u.t1 - t)); };
+    auto ask = [&](int64_t t) {
+        fetch<DT, NP>(ub, a.B, t * a.b_tok + grp * a.b_grp, a.b_tok, tokens(t), a.N, a.vec);
+        fetch<DT, NP>(uc, a.C, t * a.c_tok + grp * a.c_grp, a.c_tok, tokens(t), a.N, a.vec);
+        fetch<DT, PT>(ux, a.x, t * a.x_tok + h * a.x_head + p0, a.x_tok, tokens(t), a.P - p0, a.vec);
+    };
+    if (warp == 0) raw_steps(a, u.t0, tokens(u.t0), h, raw);
+    if (AHEAD) ask(u.t0);
     float st[StateMap<NP, PT>::CT][2][4];
     each_state<NP, PT>(st, [&](int p, int n, float& v) { v = enter && p0 + p < a.P && n < a.N ? enter[(int64_t)(p0 + p) * a.N + n] : 0.f; });
-    const float Dh = a.D ? a.D[h] : 0.f;
-    for (int i = threadIdx.x; i < PT; i += THREADS) s.bad[i] = Q;
+    if (warp == 0) {
+        chunk_steps(a, s, 0, raw, tokens(u.t0), A, bias);
+        raw_steps(a, u.t0 + Q, tokens(u.t0 + Q), h, raw);
+    }
 
-    for (int64_t t = u.t0; t < u.t1; t += Q) {
-        const int n = (int)min((int64_t)Q, u.t1 - t);
+    int buf = 0;
+    for (int64_t t = u.t0; t < u.t1; t += Q, buf ^= 1) {
+        const int n = tokens(t);
         const bool last = t + Q >= u.t1;
+        if (!AHEAD) ask(t);
         __syncthreads();
-        chunk_steps(a, s, t, n, h);
-        load_tile<DT, XP, NP, false>(s.B[0], Q * LN, LN, a.B, t * a.b_tok + grp * a.b_grp, a.b_tok, n, a.N, a.vec, nullptr);
-        load_tile<DT, XP, NP, false>(s.C[0], Q * LN, LN, a.C, t * a.c_tok + grp * a.c_grp, a.c_tok, n, a.N, a.vec, nullptr);
-        load_tile<DT, XP, PT, true>(s.x[0], Q * LP, LP, a.x, t * a.x_tok + h * a.x_head + p0, a.x_tok, n, a.P - p0, a.vec, s.bad);
+        put<DT, XP, NP, false>(s.B[0], Q * LN, LN, ub, nullptr);
+        put<DT, XP, NP, false>(s.C[0], Q * LN, LN, uc, nullptr);
+        put<DT, XP, PT, true>(s.x[0], Q * LP, LP, ux, s.bad);
         each_state<NP, PT>(st, [&](int p, int nn, float v) {
             const __nv_bfloat16 hi = __float2bfloat16_rn(v);
             s.S[0][p * LN + nn] = hi;
             if (XP > 1) s.S[XP - 1][p * LN + nn] = __float2bfloat16_rn(v - __bfloat162float(hi));
         });
         __syncthreads();
-        if (!last || a.ht) scale_x(s, pieces);
+        if (AHEAD) ask(t + Q);
+        // gates of this thread's outputs, two neighbours at a time
+        uint32_t zr[PT / 8][2];
+        if (a.z)
+#pragma unroll
+            for (int j = 0; j < PT / 8; ++j)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int i = 16 * warp + g + 8 * k, p = p0 + 8 * j + t2;
+                    const uint16_t* src = (const uint16_t*)a.z + (t + i) * a.z_tok + h * a.z_head + p;
+                    zr[j][k] = 0u;
+                    if (i >= n || p >= a.P) continue;
+                    if (a.z_pair) zr[j][k] = __ldg(reinterpret_cast<const uint32_t*>(src));
+                    else zr[j][k] = __ldg(src) | (p + 1 < a.P ? (uint32_t)__ldg(src + 1) << 16 : 0u);
+                }
+        if (!last || a.ht) scale_x(s, buf, pieces);
 
         // rows 16 warp .. +15: what the state gives them, e^{G_i} C_i S^T
         const int m0 = 16 * warp;
-        const float gi[2] = {s.G[m0 + g], s.G[m0 + g + 8]};
+        const float gi[2] = {s.G[buf][m0 + g], s.G[buf][m0 + g + 8]};
         float acc[PT / 8][4] = {};
 #pragma unroll
         for (int cp = XP - 1; cp >= 0; --cp)
@@ -334,7 +390,7 @@ __global__ void __launch_bounds__(THREADS) ssm_out_kernel(SsmArgs a) {
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         const int i = m0 + g + 8 * r, j = j0 + 8 * c + t2 + k;
-                        v[k] = j <= i ? sc[c][2 * r + k] * __expf(gi[r] - s.G[j]) * s.d[j] : 0.f;
+                        v[k] = j <= i ? sc[c][2 * r + k] * __expf(gi[r] - s.G[buf][j]) * s.d[buf][j] : 0.f;
                     }
                     const uint32_t w = pack_bf16x2(v[0], v[1]);
                     pa[0][2 * c + r] = w;
@@ -360,22 +416,38 @@ __global__ void __launch_bounds__(THREADS) ssm_out_kernel(SsmArgs a) {
 #pragma unroll
         for (int j = 0; j < PT / 8; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int i = m0 + g + 8 * (q >> 1), p = 8 * j + t2 + (q & 1);
+            for (int k = 0; k < 2; ++k) {
+                const int i = m0 + g + 8 * k, p = 8 * j + t2;
                 if (i >= n || p0 + p >= a.P) continue;
-                float xv = __bfloat162float(s.x[0][i * LP + p]);
-                if (XP > 1) xv += __bfloat162float(s.x[XP - 1][i * LP + p]);
-                float v = fmaf(Dh, xv, acc[j][q]);
-                if (i >= s.bad[p]) v = __int_as_float(0x7fc00000);
-                if (a.z) {
-                    const float zv = load16<DT>(a.z, (t + i) * a.z_tok + h * a.z_head + p0 + p);
-                    v *= zv * sigmoidf_(zv);
+                float2 xv = unpack_bf16x2(*reinterpret_cast<const uint32_t*>(&s.x[0][i * LP + p]));
+                if (XP > 1) {
+                    const float2 lo = unpack_bf16x2(*reinterpret_cast<const uint32_t*>(&s.x[XP - 1][i * LP + p]));
+                    xv.x += lo.x; xv.y += lo.y;
                 }
-                Elem<DT>::st(a.y, (size_t)(((t + i) * a.H + h) * a.P + p0 + p), v);
+                float2 v = make_float2(fmaf(Dh, xv.x, acc[j][2 * k]), fmaf(Dh, xv.y, acc[j][2 * k + 1]));
+                if (i >= s.bad[p]) v.x = __int_as_float(0x7fc00000);
+                if (i >= s.bad[p + 1]) v.y = __int_as_float(0x7fc00000);
+                if (a.z) {
+                    const float2 z = DT == LAMPA_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&zr[j][k])) : unpack_bf16x2(zr[j][k]);
+                    v.x *= z.x * sigmoidf_(z.x);
+                    v.y *= z.y * sigmoidf_(z.y);
+                }
+                const size_t at = (size_t)(((t + i) * a.H + h) * a.P + p0 + p);
+                if (a.y_pair) {
+                    if (DT == LAMPA_F16) *reinterpret_cast<__half2*>((__half*)a.y + at) = __floats2half2_rn(v.x, v.y);
+                    else *reinterpret_cast<uint32_t*>((__nv_bfloat16*)a.y + at) = pack_bf16x2(v.x, v.y);
+                } else {
+                    Elem<DT>::st(a.y, at, v.x);
+                    if (p0 + p + 1 < a.P) Elem<DT>::st(a.y, at + 1, v.y);
+                }
             }
+        if (warp == 0 && !last) {
+            chunk_steps(a, s, buf ^ 1, raw, tokens(t + Q), A, bias);
+            raw_steps(a, t + 2 * Q, tokens(t + 2 * Q), h, raw);
+        }
         if (last && !(single && a.ht)) break;
         __syncthreads();
-        update_state(st, s, expf(s.G[Q - 1]), pieces);
+        update_state(st, s, expf(s.G[buf][Q - 1]), pieces);
         each_state<NP, PT>(st, [&](int p, int, float& v) { if (s.bad[p] < Q) v = __int_as_float(0x7fc00000); });
     }
     if (single && a.ht) {
