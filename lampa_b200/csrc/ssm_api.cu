@@ -22,12 +22,13 @@ bool umma_shape(const lampa_ssm_desc* d) {
     return d->dtype == LAMPA_BF16 && d->P % 8 == 0 && d->N % 8 == 0 && d->N <= 128 && !few;
 }
 
-// Tokens per block.  mma.sync: enough blocks for six CTAs to an SM; tcgen05: for one CTA (of two heads) to an SM.
+// Tokens per block.  mma.sync: enough blocks for eight CTAs to an SM, the last of every packed sequence aside (24 001 tokens in fp16, 6 heads of
+// 32 x 16: 68 us; with six and without that 80, with four 71, with two 98); tcgen05: for one CTA (of two heads) to an SM.
 int block_tokens(const lampa_ssm_desc* d, bool umma) {
     const int q = umma ? 128 : SSM_Q;
     const int64_t n_tok = (int64_t)d->B * d->T, chunks = (n_tok + q - 1) / q, slabs = (d->P + 63) / 64;
     const int64_t per = umma ? (int64_t)d->G * ((d->H / d->G + 1) / 2) * slabs : d->H * slabs;
-    const int64_t want = std::max<int64_t>(1, (umma ? 1 : 6) * sm_count() / per);
+    const int64_t want = std::max<int64_t>(1, (umma ? 1 : 8) * sm_count() / per - (umma ? 0 : d->nseq));
     return (int)std::min<int64_t>(1 << 20, std::max<int64_t>(umma ? 1 : 2, (chunks + want - 1) / want)) * q;
 }
 

@@ -169,7 +169,7 @@ struct SmA {
     uint32_t tslot;
 };
 
-template <int NPAN>
+template <int NPAN, int PIECES>
 __global__ void __launch_bounds__(THREADS, 1) ssm_state_umma_kernel(SsmArgs a, const __grid_constant__ Maps maps) {
     if (chain_wait()) return;
     extern __shared__ __align__(1024) unsigned char raw[];
@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_state_umma_kernel(SsmArgs a, c
     if (!ssm_unit(a, blockIdx.x, u) || u.outside || (u.single(a.bl) && !a.ht)) return;
     const int hpg = a.H / a.G, pairs = (hpg + 1) / 2, grp = blockIdx.y / pairs, hl = 2 * (blockIdx.y % pairs), slab = blockIdx.z * 64;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h0 = grp * hpg + hl;
-    const int chunks = (int)((u.t1 - u.t0 + UQ - 1) / UQ), pieces = a.ht ? 3 : 1;
+    const int chunks = (int)((u.t1 - u.t0 + UQ - 1) / UQ);
     if (warp == W_MMA) {
         if (lane == 0) {
             mbar_init(&s.bar[0], 1); mbar_init(&s.bar[1], 1); mbar_init(&s.in[0], 1); mbar_init(&s.in[1], 1); mbar_init(&s.drain, 1);
@@ -201,11 +201,12 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_state_umma_kernel(SsmArgs a, c
                 if (lane == 0) {
                     tc_fence_after();
                     const uint64_t da = umma_desc_mn128(smem_u32(s.B[c & 1][0]) + hf * (TILE / 2), TILE);
-                    for (int p = pieces - 1; p >= 0; --p) {
+#pragma unroll
+                    for (int p = PIECES - 1; p >= 0; --p) {
                         const uint64_t db = umma_desc_mn128(smem_u32(s.wx[hf][p][0]), TILE / 2);
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            umma_f16_ss(tm + 128 * (c & 1), adv(da, 2048 * k), adv(db, 2048 * k), id, hf || p < pieces - 1 || k);
+                            umma_f16_ss(tm + 128 * (c & 1), adv(da, 2048 * k), adv(db, 2048 * k), id, hf || p < PIECES - 1 || k);
                     }
                     umma_commit(&s.bar[hf]);
                 }
@@ -313,20 +314,26 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_state_umma_kernel(SsmArgs a, c
                 for (int i = threadIdx.x; i < (UQ - n) * 16; i += CT)
                     *reinterpret_cast<uint4*>(s.B[c & 1][(i >> 3) & 1] + swz(n + (i >> 4), i & 7)) = make_uint4(0u, 0u, 0u, 0u);
             }
+            F2 f[2][4];
+            const F2 neg = f2(-1.f);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const float w = s.w[c & 1][k][row];
+                const F2 w2 = f2(s.w[c & 1][k][row]);
                 uint4 v = *reinterpret_cast<const uint4*>(s.x[c & 1][k] + swz(row, col));
                 if (row >= n) v = make_uint4(0u, 0u, 0u, 0u);
-                const F2 w2 = f2(w), neg = f2(-1.f);
-                F2 f[4] = {mul2(unpack2(v.x), w2), mul2(unpack2(v.y), w2), mul2(unpack2(v.z), w2), mul2(unpack2(v.w), w2)};
-                for (int p = 0; p < pieces; ++p) {
-                    const uint4 o = make_uint4(pack2(f[0]), pack2(f[1]), pack2(f[2]), pack2(f[3]));
-                    *reinterpret_cast<uint4*>(s.wx[hf][p][k] + swz(r0, col)) = o;
-                    f[0] = fma2(unpack2(o.x), neg, f[0]); f[1] = fma2(unpack2(o.y), neg, f[1]);
-                    f[2] = fma2(unpack2(o.z), neg, f[2]); f[3] = fma2(unpack2(o.w), neg, f[3]);
-                }
+                f[k][0] = mul2(unpack2(v.x), w2); f[k][1] = mul2(unpack2(v.y), w2);
+                f[k][2] = mul2(unpack2(v.z), w2); f[k][3] = mul2(unpack2(v.w), w2);
             }
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint4 o = make_uint4(pack2(f[k][0]), pack2(f[k][1]), pack2(f[k][2]), pack2(f[k][3]));
+                    *reinterpret_cast<uint4*>(s.wx[hf][p][k] + swz(r0, col)) = o;
+                    if (p + 1 == PIECES) continue;
+                    f[k][0] = fma2(unpack2(o.x), neg, f[k][0]); f[k][1] = fma2(unpack2(o.y), neg, f[k][1]);
+                    f[k][2] = fma2(unpack2(o.z), neg, f[k][2]); f[k][3] = fma2(unpack2(o.w), neg, f[k][3]);
+                }
             fence_async_smem();
             tc_fence_before();
             nb_arrive<CC>(A_W + 2 * hf + (c & 1));
@@ -363,17 +370,18 @@ struct SmC {
 // z sigmoid(z) of two values.  With t = e^-|z| the denominator 1 + t lies in [1, 2], where its reciprocal is a cubic and one Newton step:
 // 1 - v p(v) = T4(2v - 3) / T4(3) with the Chebyshev polynomial T4, 1 / 577 at most, squared by the step: 3e-6.  (Through the
 // special function unit, which has a quarter of the issue rate, both the exponential and the reciprocal would bound the epilogue.)
+// The numerator z e^min(z, 0) is the larger of z and z t.
 __device__ __forceinline__ F2 silu2(F2 z) {
-    float z0, z1, t0, t1;
+    float z0, z1, m0, m1;
     f2_get(z, z0, z1);
-    t0 = ex2(-LOG2E * fabsf(z0));
-    t1 = ex2(-LOG2E * fabsf(z1));
-    const F2 v = add2(f2(t0, t1), f2(1.f));
+    const F2 t = f2(ex2(-LOG2E * fabsf(z0)), ex2(-LOG2E * fabsf(z1)));
+    const F2 v = add2(t, f2(1.f));
     F2 p = fma2(v, f2(-128.f / 577.f), f2(768.f / 577.f));
     p = fma2(p, v, f2(-1696.f / 577.f));
     p = fma2(p, v, f2(1632.f / 577.f));
     p = mul2(p, fma2(mul2(v, p), f2(-1.f), f2(2.f)));
-    return mul2(mul2(z, f2(z0 < 0.f ? t0 : 1.f, z1 < 0.f ? t1 : 1.f)), p);
+    f2_get(mul2(z, t), m0, m1);
+    return mul2(f2(fmaxf(z0, m0), fmaxf(z1, m1)), p);
 }
 
 template <int NPAN>
@@ -827,14 +835,15 @@ bool make_map3(CUtensorMap* m, const void* base, int64_t n_tok, int heads, int c
 
 template <int NPAN>
 int launch_pan(const SsmArgs& a, const Maps& maps, int units, bool states, cudaStream_t st) {
-    static std::atomic<uint64_t> ready_s{0}, ready_o{0};
+    static std::atomic<uint64_t> ready_s{0}, ready_1{0}, ready_o{0};
     static_assert(sizeof(SmA) <= MAX_SMEM && sizeof(SmC<NPAN>) <= MAX_SMEM, "tiles fit");
     const dim3 grid(units, (unsigned)(a.G * ((a.H / a.G + 1) / 2)), (a.P + 63) / 64);
     if (states) {
-        if (!allow_smem(ready_s, ssm_state_umma_kernel<NPAN>, (int)sizeof(SmA))) return LAMPA_ERR_CUDA;
+        const auto kernel = a.ht ? ssm_state_umma_kernel<NPAN, 3> : ssm_state_umma_kernel<NPAN, 1>;
+        if (!allow_smem(a.ht ? ready_s : ready_1, kernel, (int)sizeof(SmA))) return LAMPA_ERR_CUDA;
         {
             ProfScope prof("ssm_state", st);
-            if (launch_chained(ssm_state_umma_kernel<NPAN>, grid, dim3(THREADS), sizeof(SmA), st, a, maps) != cudaSuccess) return LAMPA_ERR_CUDA;
+            if (launch_chained(kernel, grid, dim3(THREADS), sizeof(SmA), st, a, maps) != cudaSuccess) return LAMPA_ERR_CUDA;
         }
         const int rc = launch_ssm_pass(a, st);
         if (rc != LAMPA_OK) return rc;
