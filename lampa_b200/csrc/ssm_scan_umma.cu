@@ -9,11 +9,11 @@
 //   Y_h += P_h x_h                128 x 64 each, K = 128                  P_h: masked, decayed scores, bf16, from tensor memory
 // All accumulators are in tensor memory (G | P | Y | S, 128 columns each), the states S in fp32 among them.
 //
-// Sixteen warps do the element work, thread = (row or state row, head, half of the 64 columns).  Three more serve them.  One issues the
+// Sixteen warps do the element work, thread = (row or state row, head, half of the 64 columns).  Four more serve them.  One issues the
 // products (and is held up while the tensor core's queue is full, so that it does nothing else).  One copies the tiles in (tiled TMA from
 // three-dimensional maps, which fill what lies beyond the head's columns with zeros) and is the only one that polls for completions: it
-// passes them on through hardware named barriers (30 cycles, where a poll costs 200 - 300).  One turns the chunks' steps into decays a
-// chunk ahead.  Waits are bounded, and the helpers walk through all their barriers whether or not one ran out, so
+// passes them on through hardware named barriers (30 cycles, where a poll costs 200 - 300).  Two, one to a head, turn the chunks'
+// steps into decays a chunk ahead (one for both was slower than the products of a chunk).  Waits are bounded, and the helpers walk through all their barriers whether or not one ran out, so
 // nobody can be left waiting; nor can anybody reach a barrier twice in one phase, because no warp is more than a chunk ahead of another.
 #include "profile.cuh"
 #include "ssm.cuh"
@@ -27,17 +27,17 @@ namespace {
 
 constexpr int UQ = 128;                           // tokens per chunk
 constexpr int CWARPS = 16, CT = CWARPS * 32;      // element warps
-constexpr int W_MMA = CWARPS, W_CTL = CWARPS + 1, W_TAB = CWARPS + 2;     // products; copies and completions; steps
-constexpr int THREADS = CT + 96;                  // (three helpers: with a fourth an element thread would have 96 registers, not 104)
+constexpr int W_MMA = CWARPS, W_CTL = CWARPS + 1, W_TAB = CWARPS + 2;     // products; copies and completions; steps of the two heads
+constexpr int THREADS = CT + 128;
 constexpr int TILE = 16384;                       // [128][64] bf16
 constexpr float LOG2E = 1.4426950408889634f;
 
 // tensor-memory columns
 constexpr int TM_G = 0, TM_P = 128, TM_Y = 256, TM_S = 384;
 
-// named barriers of the element warps with one helper (CC), with the copying and the step warp (CS), with everybody (ALL), and of two
+// named barriers of the element warps with one helper (CC), with the copying and the step warps (CS), with everybody (ALL), and of two
 // helpers (HH)
-constexpr int CC = CT + 32, CS = CT + 64, ALL = THREADS, HH = 64;
+constexpr int CC = CT + 32, CS = CT + 96, ALL = THREADS, HH = 64;
 template <int N> __device__ __forceinline__ void nb_sync(int id) { asm volatile("bar.sync %0, %1;\n" :: "r"(id), "n"(N) : "memory"); }
 template <int N> __device__ __forceinline__ void nb_arrive(int id) { asm volatile("bar.arrive %0, %1;\n" :: "r"(id), "n"(N) : "memory"); }
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x)); return y; }
@@ -55,70 +55,60 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
 // Per head and chunk, by token: G (log2), d, d e^{G_end(32-block) - G}, d e^{G_last - G}
 struct Tab { float G[UQ], d[UQ], cf[UQ], w[UQ]; };
 
-// One warp, four tokens to a lane, both heads; tokens from n on have d = 0.  g2: log2 of the chunk's decay.  The exponent of w is summed
-// from the chunk's end, so that its error is one of its own size.
-struct Steps { float A2[2], bias[2]; int h[2]; bool has[2]; };
-__device__ __forceinline__ Steps steps_of(const SsmArgs& a, int h0, bool second) {
-    Steps p;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        p.has[k] = k == 0 || second;
-        p.h[k] = p.has[k] ? h0 + k : h0;
-        p.A2[k] = a.A[p.h[k]] * LOG2E;
-        p.bias[k] = a.dt_bias ? a.dt_bias[p.h[k]] : 0.f;
+// One warp, four tokens to a lane, one head.  The steps are asked for a chunk ahead (raw); tokens from n on have d = 0.  Returns log2 of the
+// chunk's decay.  The exponent of w is summed from the chunk's end, so that its error is one of its own size.
+struct Steps {
+    float A2, bias;
+    int h;
+    bool has;
+    uint32_t raw[4];
+    __device__ __forceinline__ Steps(const SsmArgs& a, int h0, int x, bool there) : h(there ? h0 + x : h0), has(there) {
+        A2 = a.A[h] * LOG2E;
+        bias = a.dt_bias ? a.dt_bias[h] : 0.f;
     }
-    return p;
-}
-template <bool FULL>
-__device__ __forceinline__ void make_tabs(const SsmArgs& a, const Steps& p, float* const (&ws)[2], Tab* s, int64_t t, int n, float (&g2)[2]) {
-    const int l = threadIdx.x & 31;
-    float d[2][4], g[2][4], up[2] = {0.f, 0.f}, down[2];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int64_t at = (t + min(4 * l + k, n - 1)) * a.dt_tok;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) d[x][k] = a.dt_dt == LAMPA_F32 ? __ldg((const float*)a.dt + at + p.h[x]) : __uint_as_float((uint32_t)__ldg((const uint16_t*)a.dt + at + p.h[x]));
-    }
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
+    __device__ __forceinline__ void ask(const SsmArgs& a, int64_t t, int n) {      // n <= 0: there is no such chunk
+        if (n <= 0) return;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            float v = d[x][k];
-            if (a.dt_dt == LAMPA_BF16) v = __uint_as_float(__float_as_uint(v) << 16);
-            else if (a.dt_dt == LAMPA_F16) v = __half2float(__ushort_as_half((unsigned short)__float_as_uint(v)));
-            const bool in = 4 * l + k < n && p.has[x];
-            d[x][k] = in ? ssm_step_size(v + p.bias[x], a.softplus) : 0.f;
-            g[x][k] = in ? d[x][k] * p.A2[x] : 0.f;
-            up[x] += g[x][k];
+            const int64_t at = (t + min(4 * (int)(threadIdx.x & 31) + k, n - 1)) * a.dt_tok + h;
+            raw[k] = a.dt_dt == LAMPA_F32 ? __ldg((const uint32_t*)a.dt + at) : __ldg((const uint16_t*)a.dt + at);
         }
-    down[0] = up[0]; down[1] = up[1];
+    }
+    template <bool FULL>
+    __device__ __forceinline__ float make(const SsmArgs& a, float* ws, Tab* s, int n) const {
+        const int l = threadIdx.x & 31;
+        float d[4], g[4], up = 0.f;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const float u = __shfl_up_sync(0xffffffffu, up[x], o), v = __shfl_down_sync(0xffffffffu, down[x], o);
-            if (l >= o) up[x] += u;
-            if (l + o < 32) down[x] += v;
+        for (int k = 0; k < 4; ++k) {
+            const bool in = 4 * l + k < n && has;
+            d[k] = in ? ssm_step_size(load_as_float(&raw[k], 0, a.dt_dt) + bias, a.softplus) : 0.f;
+            g[k] = in ? d[k] * A2 : 0.f;
+            up += g[k];
         }
+        float down = up;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-        const float before = __shfl_up_sync(0xffffffffu, up[x], 1), after = __shfl_down_sync(0xffffffffu, down[x], 1);
+        for (int o = 1; o < 32; o <<= 1) {
+            const float u = __shfl_up_sync(0xffffffffu, up, o), v = __shfl_down_sync(0xffffffffu, down, o);
+            if (l >= o) up += u;
+            if (l + o < 32) down += v;
+        }
+        const float before = __shfl_up_sync(0xffffffffu, up, 1), after = __shfl_down_sync(0xffffffffu, down, 1);
         float e = l < 31 ? after : 0.f, w[4];
 #pragma unroll
-        for (int k = 3; k >= 0; --k) { w[k] = d[x][k] * exp2f(e); e += g[x][k]; }
-        *reinterpret_cast<float4*>(ws[x] + 4 * l) = make_float4(w[0], w[1], w[2], w[3]);
+        for (int k = 3; k >= 0; --k) { w[k] = d[k] * exp2f(e); e += g[k]; }
+        *reinterpret_cast<float4*>(ws + 4 * l) = make_float4(w[0], w[1], w[2], w[3]);
         if (FULL) {
             float G[4], b = l ? before : 0.f;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) { b += g[x][k]; G[k] = b; }
+            for (int k = 0; k < 4; ++k) { b += g[k]; G[k] = b; }
             const float end = __shfl_sync(0xffffffffu, G[3], l | 7);
-            *reinterpret_cast<float4*>(&s[x].G[4 * l]) = make_float4(G[0], G[1], G[2], G[3]);
-            *reinterpret_cast<float4*>(&s[x].d[4 * l]) = make_float4(d[x][0], d[x][1], d[x][2], d[x][3]);
-            *reinterpret_cast<float4*>(&s[x].cf[4 * l]) = make_float4(d[x][0] * ex2(end - G[0]), d[x][1] * ex2(end - G[1]), d[x][2] * ex2(end - G[2]), d[x][3] * ex2(end - G[3]));
+            *reinterpret_cast<float4*>(&s->G[4 * l]) = make_float4(G[0], G[1], G[2], G[3]);
+            *reinterpret_cast<float4*>(&s->d[4 * l]) = make_float4(d[0], d[1], d[2], d[3]);
+            *reinterpret_cast<float4*>(&s->cf[4 * l]) = make_float4(d[0] * ex2(end - G[0]), d[1] * ex2(end - G[1]), d[2] * ex2(end - G[2]), d[3] * ex2(end - G[3]));
         }
-        g2[x] = __shfl_sync(0xffffffffu, up[x], 31);
+        return __shfl_sync(0xffffffffu, up, 31);
     }
-}
+};
 
 // State elements of a thread: row n and PC columns p0 ..  With N <= 64 the second half of dS's rows repeats the first (B's panel is there
 // twice), and its warps take the other half of the columns.
@@ -271,18 +261,20 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_state_umma_kernel(SsmArgs a, c
         nb_sync<ALL>(0);
         return;
     }
-    if (warp == W_TAB) {
-        const Steps p = steps_of(a, h0, hl + 1 < hpg);
-        float log_dec[2] = {0.f, 0.f}, g[2];
+    if (warp >= W_TAB) {
+        const int x = warp - W_TAB;
+        Steps p(a, h0, x, hl + x < hpg);
+        auto rows = [&](int c) { return (int)max((int64_t)0, min((int64_t)UQ, u.t1 - (u.t0 + (int64_t)c * UQ))); };
+        float log_dec = 0.f;
+        p.ask(a, u.t0, rows(0));
         for (int c = 0; c < chunks; ++c) {
-            const int64_t t = u.t0 + (int64_t)c * UQ;
-            float* const ws[2] = {s.w[c & 1][0], s.w[c & 1][1]};
-            make_tabs<false>(a, p, ws, nullptr, t, (int)min((int64_t)UQ, u.t1 - t), g);
-            if (lane < 2) s.tot[c & 3][lane] = exp2f(lane ? g[1] : g[0]);
-            log_dec[0] += g[0]; log_dec[1] += g[1];
+            const float g = p.make<false>(a, s.w[c & 1][x], nullptr, rows(c));
+            if (lane == 0) s.tot[c & 3][x] = exp2f(g);
+            log_dec += g;
+            p.ask(a, u.t0 + (int64_t)(c + 1) * UQ, rows(c + 1));
             nb_sync<CS>(A_NEXT);
         }
-        if (lane < 2 && (lane == 0 || p.has[1]) && slab == 0) a.blk_dec[(int64_t)blockIdx.x * a.H + h0 + lane] = lane ? log_dec[1] : log_dec[0];
+        if (p.has && lane == 0 && slab == 0) a.blk_dec[(int64_t)blockIdx.x * a.H + h0 + x] = log_dec;
         nb_sync<ALL>(0);
         return;
     }
@@ -534,14 +526,11 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a, con
             tc_fence_before();
             nb_arrive<CC>(C_G);
             if (lane == 0) {
-                if (a.z_vec) wait(&s.in_z, c);
                 wait(&s.y, c);
                 if (more && !dead) { load_C(c + 1); ++asked_c; }
             }
             __syncwarp();
-            tc_fence_before();
-            nb_arrive<CC>(C_Y);
-            if (more) {
+            if (more) {                           // the states' operand has been read, what the chunk adds to them is there
                 if (lane == 0) {
                     wait(&s.ds, c);
                     if (!dead) { load_B(c + 1); ++asked_b; }
@@ -550,6 +539,10 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a, con
                 tc_fence_before();
                 nb_arrive<CS>(C_DS);
             }
+            if (lane == 0 && a.z_vec) wait(&s.in_z, c);
+            __syncwarp();
+            tc_fence_before();
+            nb_arrive<CC>(C_Y);
             if (lane == 0) {
                 wait(&s.px, c);
                 if (more && !dead) { load_x(c + 1); ++asked_x; }
@@ -568,14 +561,15 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a, con
         nb_sync<ALL>(0);
         return;
     }
-    if (warp == W_TAB) {
-        const Steps p = steps_of(a, h0, hl + 1 < hpg);
+    if (warp >= W_TAB) {
+        const int x = warp - W_TAB;
+        Steps p(a, h0, x, hl + x < hpg);
+        auto rows = [&](int c) { return (int)max((int64_t)0, min((int64_t)UQ, u.t1 - (u.t0 + (int64_t)c * UQ))); };
+        p.ask(a, u.t0, rows(0));
         for (int c = 0; c < chunks; ++c) {
-            const int64_t t = u.t0 + (int64_t)c * UQ;
-            float* const ws[2] = {s.tab[c & 1][0].w, s.tab[c & 1][1].w};
-            float g[2];
-            make_tabs<true>(a, p, ws, s.tab[c & 1], t, (int)min((int64_t)UQ, u.t1 - t), g);
-            if (lane < 2) s.tot[c & 1][lane] = exp2f(lane ? g[1] : g[0]);
+            const float g = p.make<true>(a, s.tab[c & 1][x].w, &s.tab[c & 1][x], rows(c));
+            if (lane == 0) s.tot[c & 1][x] = exp2f(g);
+            p.ask(a, u.t0 + (int64_t)(c + 1) * UQ, rows(c + 1));
             __syncwarp();
             nb_arrive<CS>(C_DS);                  // the states that enter chunk c may be decayed for what it adds
             nb_sync<ALL>(C_NEXT);
@@ -712,6 +706,22 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a, con
                 tm_st8(tl + TM_P + 64 * hd + 16 * b + j0 / 2, o);
             }
         }
+        // ---- states
+        if (!last) {
+            nb_sync<CS>(C_DS);
+            tc_fence_after();
+            const float dec = s.tot[(c + 1) & 1][hd];
+            float v[PC / 16][16];
+#pragma unroll
+            for (int k = 0; k < PC / 16; ++k) tmem_ld16_issue(v[k], tl + TM_S + 64 * hd + own.p0 + 16 * k);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < PC / 16; ++k) {
+                tmem_loaded(v[k]);
+                put_state(k, v[k], dec);
+            }
+            fence_async_smem();
+        }
         // ---- e^{G_i} C S^T + D x (elements that are not finite, zero by now, make no difference: their rows become NaN)
         nb_sync<CC>(C_Y);
         tc_fence_after();
@@ -744,41 +754,26 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a, con
         tc_fence_before();
         fence_async_smem();                       // (zeroed elements of x)
         nb_arrive<CC>(C_P);
-        // ---- states
-        if (!last) {
-            nb_sync<CS>(C_DS);
-            tc_fence_after();
-            const float dec = s.tot[(c + 1) & 1][hd];
-            float v[PC / 16][16];
-#pragma unroll
-            for (int k = 0; k < PC / 16; ++k) tmem_ld16_issue(v[k], tl + TM_S + 64 * hd + own.p0 + 16 * k);
-            tmem_wait_ld();
-#pragma unroll
-            for (int k = 0; k < PC / 16; ++k) {
-                tmem_loaded(v[k]);
-                put_state(k, v[k], dec);
-            }
-            fence_async_smem();
-        }
-        // ---- gate, while the products run
+        // ---- gate, of the first half of the columns while the products run
         F2 gate[16];
-        if (a.z) {
+        auto gates = [&](int k) {
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
+            for (int v = 0; v < 2; ++v) {
                 uint32_t zw[4];
                 if (a.z_vec) {
-                    const uint4 z = *reinterpret_cast<const uint4*>(s.z[hd] + (at0 ^ (v << 4)));
+                    const uint4 z = *reinterpret_cast<const uint4*>(s.z[hd] + (at0 ^ ((2 * k + v) << 4)));
                     zw[0] = z.x; zw[1] = z.y; zw[2] = z.z; zw[3] = z.w;
                 } else {                          // rows that do not begin on 16-byte boundaries
-                    const int p = slab + 32 * half + 8 * v;
+                    const int p = slab + 32 * half + 16 * k + 8 * v;
                     const uint16_t* src = (const uint16_t*)a.z + (u.t0 + (int64_t)c * UQ + row) * a.z_tok + h * a.z_head + p;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) zw[e] = has && row < n && p < a.P ? (uint32_t)__ldg(src + 2 * e) | (uint32_t)__ldg(src + 2 * e + 1) << 16 : 0u;
                 }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) gate[4 * v + e] = silu2(unpack2(zw[e]));
+                for (int e = 0; e < 4; ++e) gate[8 * k + 4 * v + e] = silu2(unpack2(zw[e]));
             }
-        }
+        };
+        if (a.z) { gates(0); gates(1); }
         // ---- output, into z's place
         nb_sync<CC>(C_PX);
         tc_fence_after();
