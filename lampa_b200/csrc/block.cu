@@ -28,6 +28,8 @@ struct ConvArgsR {
     int nseq, D, W, silu, w_dt, write, groups, run;
 };
 
+__device__ __forceinline__ float exp2_approx(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x)); return y; }
+
 template <int DT> struct Bits { using T = uint16_t; };
 template <> struct Bits<LAMPA_F32> { using T = uint32_t; };
 
@@ -45,8 +47,8 @@ __device__ __forceinline__ void to_float(const typename RawRow<DT, VEC>::T& raw,
     else unpack4(raw, v, DT);
 }
 
-// 61 440 x 1 280 in bf16 (315 MB): 87 us, 55 % of the measured bandwidth; what is left is instructions (two of the special function unit per
-// element for SiLU, 36 us of its own) and the loads in flight that 100 registers leave room for.  Eight channels to a thread: 129 us.
+// 61 440 x 1 280 in bf16 (315 MB): 64 us, 75 % of the measured bandwidth (SiLU alone takes the special function unit 36).  Eight channels to a
+// thread: 129 us, one weight to a load: 211.
 template <int DT, int VEC, int MW, bool EXACT>    // MW: compile-time bound on the number of taps; EXACT: it is their number, four, and weights are 16-bit
 __global__ void __launch_bounds__(128) conv_resume_kernel(ConvArgsR a) {
     if (chain_wait()) return;
@@ -59,11 +61,21 @@ __global__ void __launch_bounds__(128) conv_resume_kernel(ConvArgsR a) {
     if (t_begin >= a.n_tok) return;
     const int W = EXACT ? MW : a.W;
     const int64_t t_end = min(t_begin + a.run, a.n_tok);
-    constexpr int AHEAD = 4;          // rows of a batch; the next batch is asked for before the first is used
-    Raw raw[2][AHEAD];
-    auto ask = [&](int buf, int64_t t0) {
+    // Rows come in batches of four through a ring of this thread's own in shared memory (registers for three batches in flight would halve
+    // the threads, and with one in flight the loads bound it: 84 us); single channels, which are too small to copy that way, through registers.
+    constexpr int AHEAD = 4, RING = VEC > 1 ? 4 : 1;
+    __shared__ Raw ring[RING][AHEAD][VEC > 1 ? 128 : 1];
+    auto ask = [&](int slot, int64_t t0, int64_t end) {
+        if constexpr (VEC > 1) {
+            if (t0 < end)
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k) raw[buf][k] = load_raw<DT, VEC>(a.x, min(t0 + k, a.n_tok - 1) * a.x_tok + d0);
+                for (int k = 0; k < AHEAD; ++k) {
+                    const void* src = (const typename Elem<DT>::T*)a.x + min(t0 + k, a.n_tok - 1) * a.x_tok + d0;
+                    if constexpr (sizeof(Raw) == 16) asm volatile("cp.async.ca.shared.global [%0], [%1], 16;\n" :: "r"(smem_u32(&ring[slot][k][threadIdx.x])), "l"(src) : "memory");
+                    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" :: "r"(smem_u32(&ring[slot][k][threadIdx.x])), "l"(src) : "memory");
+                }
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
+        }
     };
     int seq;                          // sequence of the first token; nseq: behind the last one
     int64_t bos, eos;
@@ -90,7 +102,10 @@ __global__ void __launch_bounds__(128) conv_resume_kernel(ConvArgsR a) {
     if (!bounds() || t_begin < bos) return;
     // tokens that look back into the cache of a sequence of an earlier run are that run's
     const int64_t t_first = bos < t_begin ? max(t_begin, min(eos, bos + W - 1)) : t_begin;
-    ask(0, t_first);
+    // (a sequence that opens in the last batch may move the end by W - 1)
+    const int64_t ask_end = t_end + W - 1;
+#pragma unroll
+    for (int i = 0; i < RING - 1; ++i) ask(i, t_first + i * AHEAD, ask_end);
 
     float wt[MW][VEC], bs[VEC];
     if constexpr (EXACT && VEC == 4) {             // a thread's weights are 4 MW neighbours
@@ -142,6 +157,25 @@ __global__ void __launch_bounds__(128) conv_resume_kernel(ConvArgsR a) {
     auto token = [&](const Raw& row, int64_t at, bool inside) {
         float cur[VEC], out[VEC];
         to_float<DT, VEC>(row, cur);
+        if constexpr (VEC == 4) {                                  // two channels to an instruction
+#pragma unroll
+            for (int j = 0; j < 4; j += 2) {
+                F2 acc = f2(bs[j], bs[j + 1]);
+#pragma unroll
+                for (int i = 0; i < MW - 1; ++i)
+                    if (i < W - 1) acc = fma2(f2(win[i][j], win[i][j + 1]), f2(wt[i][j], wt[i][j + 1]), acc);
+#pragma unroll
+                for (int i = 0; i < MW; ++i)
+                    if (i == W - 1) acc = fma2(f2(cur[j], cur[j + 1]), f2(wt[i][j], wt[i][j + 1]), acc);
+                if (a.silu) {
+                    float e0, e1;
+                    f2_get(mul2(acc, f2(-1.4426950408889634f)), e0, e1);
+                    f2_get(add2(f2(exp2_approx(e0), exp2_approx(e1)), f2(1.f)), e0, e1);
+                    acc = mul2(acc, f2(rcp_approx(e0), rcp_approx(e1)));
+                }
+                f2_get(acc, out[j], out[j + 1]);
+            }
+        } else
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
             float acc = bs[j];
@@ -153,9 +187,7 @@ __global__ void __launch_bounds__(128) conv_resume_kernel(ConvArgsR a) {
                 if (i == W - 1) acc = fmaf(cur[j], wt[i][j], acc);
             out[j] = acc;
         }
-        if (a.silu)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) out[j] *= sigmoid_fast(out[j]);
+        if (VEC == 1 && a.silu) out[0] *= sigmoid_fast(out[0]);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) out[j] = inside ? out[j] : 0.f;
         if constexpr (VEC == 1) Elem<DT>::st(a.y, (size_t)at, out[0]);
@@ -167,39 +199,47 @@ __global__ void __launch_bounds__(128) conv_resume_kernel(ConvArgsR a) {
                 if (i < W - 2) win[i][j] = win[i + 1 < MW ? i + 1 : i][j];
                 else if (i == W - 2) win[i][j] = cur[j];
     };
+    int slot = 0;
 #pragma unroll 1
-    for (int64_t t1 = t_first; t1 < t_stop; t1 += 2 * AHEAD) {
+    for (int64_t t0 = t_first; t0 < t_stop; t0 += AHEAD, slot = (slot + 1) % RING) {
+        Raw raw[AHEAD];
+        if constexpr (VEC > 1) {
+            ask((slot + RING - 1) % RING, t0 + (RING - 1) * AHEAD, ask_end);
+            asm volatile("cp.async.wait_group %0;\n" :: "n"(RING - 1) : "memory");
 #pragma unroll
-        for (int buf = 0; buf < 2; ++buf) {
-            const int64_t t0 = t1 + buf * AHEAD;
-            if (t0 + AHEAD < t_end + W - 1) ask(buf ^ 1, t0 + AHEAD);      // (a sequence that opens in this batch may move t_stop that far)
-            if (t0 + AHEAD <= min(eos, t_stop) && seq < a.nseq) {          // a whole batch of one sequence
+            for (int k = 0; k < AHEAD; ++k) raw[k] = ring[slot][k][threadIdx.x];
+        } else {
 #pragma unroll
-                for (int k = 0; k < AHEAD; ++k) token(raw[buf][k], (t0 + k) * a.D + d0, true);
-                continue;
-            }
+            for (int k = 0; k < AHEAD; ++k) raw[k] = load_raw<DT, VEC>(a.x, min(t0 + k, a.n_tok - 1) * a.x_tok + d0);
+        }
+        if (t0 + AHEAD <= min(eos, t_stop) && seq < a.nseq) {              // a whole batch of one sequence
 #pragma unroll
-            for (int k = 0; k < AHEAD; ++k) {
-                const int64_t t = t0 + k;
+            for (int k = 0; k < AHEAD; ++k) token(raw[k], (t0 + k) * a.D + d0, true);
+            continue;
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const int64_t t = t0 + k;
+            if (t >= t_stop) break;
+            if (t >= eos) {                                        // the next sequence that has tokens, or what lies behind the last
+                do { ++seq; } while (seq < a.nseq && a.cu && a.cu[seq + 1] <= t);
+                if (!bounds() || bos != t) t_stop = t;             // (bad offsets: nothing more)
                 if (t >= t_stop) break;
-                if (t >= eos) {                                    // the next sequence that has tokens, or what lies behind the last
-                    do { ++seq; } while (seq < a.nseq && a.cu && a.cu[seq + 1] <= t);
-                    if (!bounds() || bos != t) return;
-                    history(t);
-                }
-                token(raw[buf][k], t * a.D + d0, seq < a.nseq);
+                history(t);
             }
+            token(raw[k], t * a.D + d0, seq < a.nseq);
         }
     }
+    if constexpr (VEC > 1) asm volatile("cp.async.wait_all;\n" ::: "memory");
 }
 
 template <int DT, int VEC>
 int launch_conv(ConvArgsR a, bool vec_w, cudaStream_t st) {
     a.groups = (a.D + VEC - 1) / VEC;
-    // 32 tokens where that leaves every SM a thousand threads (fewer weights and earlier rows to a token: 87 instead of 100 us for
-    // 61 440 x 1 280 in bf16, 94 with 128), else 16 (7.7 instead of 9.6 us for 6 007 x 640)
+    // 64 or 32 tokens where that leaves every SM a thousand threads (fewer weights and earlier rows to a token: 64 instead of 67 us with 64
+    // instead of 32 for 61 440 x 1 280 in bf16), else 16 (7.7 instead of 9.6 us with 32 for 6 007 x 640)
     a.run = RUN_MIN;
-    while (a.run < 32 && a.n_tok * a.groups / (2 * a.run) >= (int64_t)sm_count() * 1024) a.run *= 2;
+    while (a.run < 64 && a.n_tok * a.groups / (2 * a.run) >= (int64_t)sm_count() * 1024) a.run *= 2;
     const int64_t runs = (a.n_tok + a.run - 1) / a.run, grid = (runs * a.groups + 127) / 128;
     if (grid > INT32_MAX) return LAMPA_ERR_UNSUPPORTED;
     auto kernel = conv_resume_kernel<DT, VEC, 8, false>;

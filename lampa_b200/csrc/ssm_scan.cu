@@ -246,11 +246,14 @@ __global__ void __launch_bounds__(THREADS) ssm_state_kernel(SsmArgs a) {
 }
 
 // Over the blocks of a sequence: what enters each of them takes the place of what it makes of an empty state.  Also the final state,
-// but for sequences of one block, whose only CTA writes it.
+// but for sequences of one block, whose only CTA writes it.  V state elements to a thread, AHEAD blocks asked for before the first is used
+// (one by one: 27 us instead of 5 for 18 blocks of 16 heads of 64 x 128).
+template <int V, int AHEAD>
 __global__ void __launch_bounds__(256) ssm_pass_kernel(SsmArgs a) {
     if (chain_wait()) return;
-    const int pn = a.P * a.N, slabs = (pn + 255) / 256, seq = blockIdx.x / slabs, h = blockIdx.y;
-    const int e = (blockIdx.x - seq * slabs) * 256 + threadIdx.x;
+    struct alignas(4 * V) Vec { float v[V]; };
+    const int pn = a.P * a.N, slabs = (pn / V + 255) / 256, seq = blockIdx.x / slabs, h = blockIdx.y;
+    const int e = ((blockIdx.x - seq * slabs) * 256 + threadIdx.x) * V;
     int64_t bos = (int64_t)seq * a.T, eos = bos + a.T, u0 = (int64_t)seq * a.nb;
     if (a.cu) {
         bos = a.cu[seq]; eos = a.cu[seq + 1];
@@ -259,28 +262,33 @@ __global__ void __launch_bounds__(256) ssm_pass_kernel(SsmArgs a) {
     }
     if (e >= pn) return;
     const int64_t len = eos - bos, out = ((int64_t)seq * a.H + h) * pn + e;
-    float s = a.h0 ? a.h0[out] : 0.f;
+    Vec s = {};
+    if (a.h0) s = *reinterpret_cast<const Vec*>(a.h0 + out);
     if (len > a.bl || (a.whole && a.ht && len > 0)) {
         const int nb = (int)((len + a.bl - 1) / a.bl);
         float* p = a.blk + (u0 * a.H + h) * pn + e;
         const float* dec = a.blk_dec + u0 * a.H + h;
         const int64_t step = (int64_t)a.H * pn;
-        for (int b = 0; b < nb; b += 8) {                          // eight blocks are asked for before the first is used
-            float part[8], e[8];
+        for (int b = 0; b < nb; b += AHEAD) {
+            Vec part[AHEAD];
+            float d[AHEAD];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                part[k] = b + k < nb ? p[(b + k) * step] : 0.f;
-                e[k] = b + k < nb ? dec[(int64_t)(b + k) * a.H] : 0.f;
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
+            for (int k = 0; k < AHEAD; ++k)
                 if (b + k < nb) {
-                    p[(b + k) * step] = s;
-                    s = fmaf(exp2f(e[k]), s, part[k]);
+                    part[k] = *reinterpret_cast<const Vec*>(p + (b + k) * step);
+                    d[k] = dec[(int64_t)(b + k) * a.H];
+                }
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k)
+                if (b + k < nb) {
+                    *reinterpret_cast<Vec*>(p + (b + k) * step) = s;
+                    const float x = exp2f(d[k]);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) s.v[i] = fmaf(x, s.v[i], part[k].v[i]);
                 }
         }
     } else if (len > 0) return;
-    if (a.ht) a.ht[out] = s;
+    if (a.ht) *reinterpret_cast<Vec*>(a.ht + out) = s;
 }
 
 template <int DT, int NP, int PT>
@@ -500,10 +508,13 @@ int launch_any(const SsmArgs& a, int units, bool blocks, cudaStream_t st) {
 }  // namespace
 
 int launch_ssm_pass(const SsmArgs& a, cudaStream_t st) {
-    const int64_t slabs = ((int64_t)a.P * a.N + 255) / 256;
+    // four elements to a thread where they fill the GPU all the same
+    const bool vec = (int64_t)a.P * a.N * a.nseq * a.H >= (int64_t)sm_count() * 2048 && (int64_t)a.P * a.N % 4 == 0 && (((uintptr_t)a.h0 | (uintptr_t)a.ht) & 15) == 0;
+    const int64_t slabs = ((int64_t)a.P * a.N / (vec ? 4 : 1) + 255) / 256;
     if (slabs * a.nseq > INT32_MAX) return LAMPA_ERR_UNSUPPORTED;
     ProfScope prof("ssm_pass", st);
-    return launch_chained(ssm_pass_kernel, dim3((unsigned)(slabs * a.nseq), a.H), dim3(256), 0, st, a) == cudaSuccess ? LAMPA_OK : LAMPA_ERR_CUDA;
+    return launch_chained(vec ? ssm_pass_kernel<4, 8> : ssm_pass_kernel<1, 8>, dim3((unsigned)(slabs * a.nseq), a.H), dim3(256), 0, st, a) == cudaSuccess
+               ? LAMPA_OK : LAMPA_ERR_CUDA;
 }
 
 int launch_ssm_scan_mma(const SsmArgs& a, int dtype, int units, bool blocks, cudaStream_t st) {

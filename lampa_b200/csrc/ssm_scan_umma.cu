@@ -581,7 +581,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a, con
     const int q = warp & 3, hd = warp >> 3, half = (warp >> 2) & 1, row = 32 * q + lane;
     const Own<NPAN> own(q, half, lane);
     constexpr int PC = Own<NPAN>::PC;
-    const int h = h0 + hd;
+    const int h = h0 + hd, len = (int)(u.t1 - u.t0);
     const bool has = hl + hd < hpg;
     const uint32_t tl = tm + ((uint32_t)(32 * q) << 16);
     if (threadIdx.x < 128) s.bad[threadIdx.x >> 6][threadIdx.x & 63] = UQ;
@@ -631,7 +631,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a, con
 
     for (int c = 0; c < chunks; ++c) {
         const bool last = c + 1 == chunks;
-        const int n = (int)min((int64_t)UQ, u.t1 - (u.t0 + (int64_t)c * UQ));
+        const int n = min(UQ, len - c * UQ);
         const Tab& t = s.tab[c & 1][hd];
         nb_sync<ALL>(C_NEXT);                     // x and the steps are there
         // ---- wx
