@@ -22,13 +22,13 @@ bool umma_shape(const lampa_ssm_desc* d) {
     return d->dtype == LAMPA_BF16 && d->P % 8 == 0 && d->N % 8 == 0 && d->N <= 128 && !few;
 }
 
-// Tokens per block.  mma.sync: enough blocks for eight CTAs to an SM, the last of every packed sequence aside (24 001 tokens in fp16, 6 heads of
+// Tokens per block.  mma.sync: enough blocks for eight CTAs to an SM, the last of every packed sequence aside where they are few (24 001 tokens in fp16, 6 heads of
 // 32 x 16: 68 us; with six and without that 80, with four 71, with two 98); tcgen05: for one CTA (of two heads) to an SM.
 int block_tokens(const lampa_ssm_desc* d, bool umma) {
     const int q = umma ? 128 : SSM_Q;
     const int64_t n_tok = (int64_t)d->B * d->T, chunks = (n_tok + q - 1) / q, slabs = (d->P + 63) / 64;
     const int64_t per = umma ? (int64_t)d->G * ((d->H / d->G + 1) / 2) * slabs : d->H * slabs;
-    const int64_t want = std::max<int64_t>(1, (umma ? 1 : 8) * sm_count() / per - (umma ? 0 : d->nseq));
+    const int64_t all = (umma ? 1 : 8) * (int64_t)sm_count() / per, want = std::max<int64_t>(1, umma ? all : std::max(all / 4, all - d->nseq));
     return (int)std::min<int64_t>(1 << 20, std::max<int64_t>(umma ? 1 : 2, (chunks + want - 1) / want)) * q;
 }
 
@@ -69,7 +69,10 @@ extern "C" int lampa_ssm_scan(const lampa_ssm_desc* d, const void* x, int64_t x_
     if (!x || !dt || !A || !B || !C || !y) return LAMPA_ERR_ARG;
     auto rows16 = [](const void* q, int64_t s0, int64_t s1) { return (((uintptr_t)q | (uintptr_t)(s0 * 2) | (uintptr_t)(s1 * 2)) & 15) == 0; };
     const bool vec = d->P % 8 == 0 && d->N % 8 == 0 && rows16(x, x_tok, x_head) && rows16(B, b_tok, b_grp) && rows16(C, c_tok, c_grp);
-    const bool umma = umma_shape(d) && (int64_t)d->B * d->T <= INT32_MAX - 128 && vec && ((uintptr_t)y & 15) == 0 && umma_enabled();
+    const int64_t n_tok = (int64_t)d->B * d->T;
+    auto steps_on = [&](int64_t tok, int64_t head, int n) { return (n_tok == 1 || tok > 0) && (n == 1 || head > 0); };     // (a tensor map has no zero distances)
+    const bool umma = umma_shape(d) && n_tok <= INT32_MAX - 128 && vec && ((uintptr_t)y & 15) == 0 && umma_enabled() &&
+                      steps_on(x_tok, x_head, d->H) && steps_on(b_tok, b_grp, d->G) && steps_on(c_tok, c_grp, d->G);
     const Plan p = plan_of(d, umma);
     if (p.units > INT32_MAX) return LAMPA_ERR_UNSUPPORTED;
     if (p.bytes && (!ws || ws_bytes < p.bytes || ((uintptr_t)ws & 15))) return LAMPA_ERR_WORKSPACE;
@@ -81,10 +84,10 @@ extern "C" int lampa_ssm_scan(const lampa_ssm_desc* d, const void* x, int64_t x_
     a.status = status;
     a.x_tok = x_tok; a.x_head = x_head; a.z_tok = z_tok; a.z_head = z_head; a.b_tok = b_tok; a.b_grp = b_grp; a.c_tok = c_tok; a.c_grp = c_grp;
     a.dt_tok = dt_tok;
-    a.n_tok = (int64_t)d->B * d->T; a.T = d->T; a.nseq = d->nseq ? d->nseq : d->B; a.nb = p.nb; a.bl = p.bl;
+    a.n_tok = n_tok; a.T = d->T; a.nseq = d->nseq ? d->nseq : d->B; a.nb = p.nb; a.bl = p.bl;
     a.H = d->H; a.P = d->P; a.N = d->N; a.G = d->G; a.dt_dt = d->dt_dtype; a.softplus = d->dt_softplus;
     a.vec = vec;
-    a.z_vec = z && rows16(z, z_tok, z_head);
+    a.z_vec = z && rows16(z, z_tok, z_head) && steps_on(z_tok, z_head, d->H);
     a.z_pair = z && d->P % 2 == 0 && (((uintptr_t)z | (uintptr_t)(z_tok * 2) | (uintptr_t)(z_head * 2)) & 3) == 0;
     a.y_pair = d->P % 2 == 0 && ((uintptr_t)y & 3) == 0;
     a.whole = umma;

@@ -38,7 +38,7 @@ def _rows(t: Optional[torch.Tensor], aligned: bool = False) -> Optional[torch.Te
     even = t.shape[0] <= 1 or t.shape[1] <= 1 or t.stride(0) == t.shape[1] * t.stride(1)
     even = even and (t.shape[-1] <= 1 or t.stride(-1) == 1)
     if aligned:
-        even = even and not any(v * t.element_size() % 16 for v in t.stride()[:-1]) and t.data_ptr() % 16 == 0
+        even = even and not any(v * t.element_size() % 16 for n, v in zip(t.shape[:-1], t.stride()) if n > 1) and t.data_ptr() % 16 == 0
     return t if even else t.contiguous()
 
 
@@ -64,6 +64,7 @@ def state_space_scan(
     rows, as a projection's output is split (x, B and C are copied where these do not begin on 16-byte boundaries); dt may
     have a type of its own.  Any P, N up to 256, any lengths from 0 on; rows
     behind the last entry of cu_seqlens come out as zero.  D None: no skip; z None: no gate.
+    A times a step is meant to be at most 0 (a decay); growth is computed too as long as e^(A sum d) over any 128 tokens is finite.
     The last bits of y and of the states depend on how long the whole call is (the tokens are cut into blocks), those of two
     equal calls do not differ.
     Offsets on the device that fall or leave the input are reported through `check_status()`.

@@ -23,6 +23,11 @@ def lb():
     lampa_b200.check_status()
 
 
+@pytest.fixture(autouse=True)
+def _checked_by_the_tests(monkeypatch):
+    monkeypatch.setenv("LAMPA_B200_CHECK", "0")    # the status word is read below, not inside the calls
+
+
 def _near(got, ref, bound, what):
     d = (got.double() - ref).abs()
     # a value beyond the type's largest rounds to infinity of its sign, and nothing else does (65 520 and more in fp16)
@@ -167,6 +172,31 @@ def test_scan_reads_parts_of_wider_rows(lb, pitch):
     odd = dict(a, x=a["x"].transpose(2, 3).contiguous().transpose(2, 3), dt=a["dt"].transpose(1, 2).contiguous().transpose(1, 2))
     y3, h3 = lb.state_space_scan(**odd, output_final_state=True)
     assert torch.equal(y, y3) and torch.equal(ht, h3)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_scan_of_expanded_and_single_axes(lb, dtype):
+    """B and C of one group for all by a stride of zero, one x for all heads, one head or token out of many"""
+    a = scan_inputs(13, 1, 300, 4, 64, 2, 64, dtype, z=True)
+    a["B"], a["C"] = (a[k][:, :, :1].expand(1, 300, 2, 64) for k in ("B", "C"))
+    check_scan(lb, a)
+    a["x"], a["z"] = (a[k][:, :, :1].expand(1, 300, 4, 64) for k in ("x", "z"))
+    check_scan(lb, a)
+    a["x"] = a["x"][:, :1].expand(1, 300, 4, 64)
+    check_scan(lb, a)
+    a = scan_inputs(14, 1, 300, 4, 64, 2, 64, dtype, z=True, pitch=3)
+    one = dict(a, x=a["x"][:, :, 1:2], dt=a["dt"][..., 1:2], z=a["z"][:, :, 1:2], B=a["B"][:, :, 1:], C=a["C"][:, :, 1:], A=a["A"][1:2], D=a["D"][1:2], dt_bias=a["dt_bias"][1:2])
+    check_scan(lb, one)
+    check_scan(lb, {k: (v[:, 7:8] if k in ("x", "dt", "B", "C", "z") else v) for k, v in one.items()})
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_scan_many_short_sequences_and_a_long_one(lb, dtype):
+    lens = [3, 0, 1] * 90 + [2500] + [2] * 60
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    check_scan(lb, scan_inputs(15, 1, cu[-1], 6, 32, 1, 16, dtype, h0=True, nseq=len(lens)), cu)
 
 
 @pytest.mark.parametrize("dt_dtype", [F32, FP, BF])
