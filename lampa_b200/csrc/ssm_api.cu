@@ -16,7 +16,7 @@ bool built(const lampa_ssm_desc* d) {
 }
 
 // The tcgen05 kernels take bf16 rows in pieces of 16 bytes, and their state is one operand tile.  Up to 128 tokens of few heads the
-// mma.sync form is one launch that ends with the state (37 tokens, 8 heads of 64 x 64: MMA37 us; tcgen05: 20.4 in three).
+// mma.sync form is one launch that ends with the state (37 tokens, 8 heads of 64 x 64: 13.1 us; tcgen05: 20.4 in three).
 bool umma_shape(const lampa_ssm_desc* d) {
     const bool few = d->T <= 2 * SSM_Q && (int64_t)d->B * d->H * ((d->P + 63) / 64) <= 2 * sm_count();
     return d->dtype == LAMPA_BF16 && d->P % 8 == 0 && d->N % 8 == 0 && d->N <= 128 && !few;

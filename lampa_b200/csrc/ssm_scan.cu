@@ -12,6 +12,11 @@
 //
 // A token whose x is not finite must not reach the rows in front of it through a zero of the mask (0 * NaN): such elements are taken
 // out of the tile, and from their row on the column is NaN, as the recurrence has it.
+//
+// What bounds it: instructions (24 001 packed tokens in fp16, 6 heads of 32 x 16, 68 us in all: output 40 us, issue slots 44 %, tensor pipe 10 %,
+// DRAM 5 %; states 22, pass 7), most of them spent on splitting fp16 into pieces, on decays and on the gate, in four warps a CTA whose phases
+// follow one another.  With tiles and steps loaded just before their use 107 us.  61 440 bf16 tokens, 16 heads of 64 x 128, take 1 120 us here and
+// 214 in the tcgen05 form.
 #include "profile.cuh"
 #include "ssm.cuh"
 
@@ -508,8 +513,9 @@ int launch_any(const SsmArgs& a, int units, bool blocks, cudaStream_t st) {
 }  // namespace
 
 int launch_ssm_pass(const SsmArgs& a, cudaStream_t st) {
-    // four elements to a thread where they fill the GPU all the same
-    const bool vec = (int64_t)a.P * a.N * a.nseq * a.H >= (int64_t)sm_count() * 2048 && (int64_t)a.P * a.N % 4 == 0 && (((uintptr_t)a.h0 | (uintptr_t)a.ht) & 15) == 0;
+    // four elements to a thread where every SM still has 128 threads (16 heads of 64 x 128: 3.3 instead of 5.2 us; 7 sequences of 6 heads of
+    // 32 x 16: 9.3 instead of 7.3)
+    const bool vec = (int64_t)a.P * a.N * a.nseq * a.H >= (int64_t)sm_count() * 512 && (int64_t)a.P * a.N % 4 == 0 && (((uintptr_t)a.h0 | (uintptr_t)a.ht) & 15) == 0;
     const int64_t slabs = ((int64_t)a.P * a.N / (vec ? 4 : 1) + 255) / 256;
     if (slabs * a.nseq > INT32_MAX) return LAMPA_ERR_UNSUPPORTED;
     ProfScope prof("ssm_pass", st);
