@@ -28,8 +28,6 @@ namespace {
 constexpr int Q = SSM_Q;
 constexpr int THREADS = 128;
 
-__device__ __forceinline__ bool finite_(float v) { return fabsf(v) <= 3.402823466e38f; }
-
 template <int DT, int NP, int PT>
 struct Sm {
     static constexpr int XP = DT == LAMPA_F16 ? 2 : 1;                 // bf16 pieces of an input
@@ -40,7 +38,7 @@ struct Sm {
     __nv_bfloat16 x[XP][Q * LP];
     __nv_bfloat16 wx[3][Q * LP];                                       // d x e^{G_last - G}
     float G[2][Q], d[2][Q], w[2][Q];                                   // by chunk parity
-    int bad[PT];                                                       // first row of the column that is not finite, or Q
+    int bad[PT], any_bad;                                              // first row of the column that is not finite, or Q; whether there is one
 };
 
 // Rows [0, n) of a matrix of 16-bit elements as COLS-wide tile pieces of 16 bytes in a thread's registers, zero beyond n rows and `cols`
@@ -64,29 +62,69 @@ __device__ __forceinline__ void fetch(uint4 (&u)[Piece<COLS>::N], const void* ba
         }
     }
 }
-// ... into XP bf16 pieces.  FIND: elements that are not finite become zero and leave their row in bad[].
-template <int DT, int XP, int COLS, bool FIND>
-__device__ __forceinline__ void put(__nv_bfloat16* dst, int piece, int ld, const uint4 (&u)[Piece<COLS>::N], int* bad) {
+// Two 16-bit values as floats
+template <int DT>
+__device__ __forceinline__ float2 pair_of(uint32_t w) { return DT == LAMPA_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&w)) : unpack_bf16x2(w); }
+// ... into XP bf16 pieces.
+template <int DT, int XP, int COLS>
+__device__ __forceinline__ void put(__nv_bfloat16* dst, int piece, int ld, const uint4 (&u)[Piece<COLS>::N]) {
 #pragma unroll
     for (int k = 0; k < Piece<COLS>::N; ++k) {
-        const int i = threadIdx.x + THREADS * k, r = i / (COLS / 8), c = (i % (COLS / 8)) * 8;
-        uint32_t w[4] = {u[k].x, u[k].y, u[k].z, u[k].w}, lo[4];
+        const int i = threadIdx.x + THREADS * k, at = i / (COLS / 8) * ld + (i % (COLS / 8)) * 8;
+        if (XP == 1) {                                                 // bf16 as it is
+            *reinterpret_cast<uint4*>(dst + at) = u[k];
+            continue;
+        }
+        const uint32_t w[4] = {u[k].x, u[k].y, u[k].z, u[k].w};
+        uint32_t hi[4], lo[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            float2 f = DT == LAMPA_F16 ? __half22float2(*reinterpret_cast<__half2*>(&w[j])) : unpack_bf16x2(w[j]);
-            if (FIND) {
-                if (!finite_(f.x)) { atomicMin(&bad[c + 2 * j], r); f.x = 0.f; }
-                if (!finite_(f.y)) { atomicMin(&bad[c + 2 * j + 1], r); f.y = 0.f; }
-            }
-            w[j] = pack_bf16x2(f.x, f.y);
-            if (XP > 1) {
-                const float2 h = unpack_bf16x2(w[j]);
-                lo[j] = pack_bf16x2(f.x - h.x, f.y - h.y);
-            }
+            const float2 f = pair_of<DT>(w[j]);
+            hi[j] = pack_bf16x2(f.x, f.y);
+            const float2 h = unpack_bf16x2(hi[j]);
+            lo[j] = pack_bf16x2(f.x - h.x, f.y - h.y);
         }
-        *reinterpret_cast<uint4*>(dst + r * ld + c) = make_uint4(w[0], w[1], w[2], w[3]);
-        if (XP > 1) *reinterpret_cast<uint4*>(dst + piece + r * ld + c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        *reinterpret_cast<uint4*>(dst + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(dst + piece + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
+}
+// x: as it is (KEEP; elements that are not finite become zero there and leave their row in bad[]), and as `pieces` pieces of w x
+template <int DT, int NP, int PT, bool KEEP>
+__device__ __forceinline__ void put_x(Sm<DT, NP, PT>& s, int buf, uint4 (&u)[Piece<PT>::N], int pieces) {
+    using S = Sm<DT, NP, PT>;
+    constexpr uint32_t EXP = DT == LAMPA_F16 ? 0x7c007c00u : 0x7f807f80u, ONE = DT == LAMPA_F16 ? 0x04000400u : 0x00800080u;
+#pragma unroll
+    for (int k = 0; k < Piece<PT>::N; ++k) {
+        const int i = threadIdx.x + THREADS * k, r = i / (PT / 8), c = (i % (PT / 8)) * 8, at = r * S::LP + c;
+        uint32_t w[4] = {u[k].x, u[k].y, u[k].z, u[k].w};
+        const float wr = s.w[buf][r];
+        float2 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[j] = pair_of<DT>(w[j]);
+            v[j].x *= wr; v[j].y *= wr;
+        }
+        if (KEEP && ((((w[0] & EXP) + ONE) | ((w[1] & EXP) + ONE) | ((w[2] & EXP) + ONE) | ((w[3] & EXP) + ONE)) & 0x80008000u)) {
+            s.any_bad = 1;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if ((((w[j] & EXP) + ONE) & 0x8000u)) { atomicMin(&s.bad[c + 2 * j], r); w[j] &= 0xffff0000u; }
+                if ((((w[j] & EXP) + ONE) & 0x80000000u)) { atomicMin(&s.bad[c + 2 * j + 1], r); w[j] &= 0xffffu; }
+            }
+            u[k] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        for (int p = 0; p < pieces; ++p) {
+            uint32_t o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                o[j] = pack_bf16x2(v[j].x, v[j].y);
+                const float2 h = unpack_bf16x2(o[j]);
+                v[j].x -= h.x; v[j].y -= h.y;
+            }
+            *reinterpret_cast<uint4*>(&s.wx[p][at]) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+    }
+    if (KEEP) put<DT, S::XP, PT>(s.x[0], Q * S::LP, S::LP, u);
 }
 
 // d, G and w = d e^{G_last - G} of a chunk's n tokens (tokens beyond them have d = 0), by the first warp, two tokens to a lane: raw steps a
@@ -121,27 +159,6 @@ __device__ __forceinline__ void chunk_steps(const SsmArgs& a, SM& s, int buf, co
     s.G[buf][2 * l] = b + g[0]; s.G[buf][2 * l + 1] = up;
     s.w[buf][2 * l] = d[0] * expf(e + g[1]);
     s.w[buf][2 * l + 1] = d[1] * expf(e);
-}
-
-// wx pieces from the x tile: `pieces` of three
-template <int DT, int NP, int PT>
-__device__ __forceinline__ void scale_x(Sm<DT, NP, PT>& s, int buf, int pieces) {
-    using S = Sm<DT, NP, PT>;
-    for (int i = threadIdx.x; i < Q * (PT / 2); i += THREADS) {
-        const int r = i / (PT / 2), c = (i % (PT / 2)) * 2, at = r * S::LP + c;
-        float2 v = unpack_bf16x2(*reinterpret_cast<const uint32_t*>(&s.x[0][at]));
-        if (S::XP > 1) {
-            const float2 lo = unpack_bf16x2(*reinterpret_cast<const uint32_t*>(&s.x[S::XP - 1][at]));
-            v.x += lo.x; v.y += lo.y;
-        }
-        v.x *= s.w[buf][r]; v.y *= s.w[buf][r];
-        for (int p = 0; p < pieces; ++p) {
-            const uint32_t u = pack_bf16x2(v.x, v.y);
-            *reinterpret_cast<uint32_t*>(&s.wx[p][at]) = u;
-            const float2 h = unpack_bf16x2(u);
-            v.x -= h.x; v.y -= h.y;
-        }
-    }
 }
 
 // The state of a CTA: PT x NP, warp w holds rows 16 (w % RS) .. +15 and columns of 16 (cg + CG i)
@@ -229,16 +246,14 @@ __global__ void __launch_bounds__(THREADS) ssm_state_kernel(SsmArgs a) {
     for (int64_t t = u.t0; t < u.t1; t += Q, buf ^= 1) {
         if (!AHEAD) ask(t);
         __syncthreads();
-        put<DT, SMT::XP, NP, false>(s.B[0], Q * SMT::LN, SMT::LN, ub, nullptr);
-        put<DT, SMT::XP, PT, false>(s.x[0], Q * SMT::LP, SMT::LP, ux, nullptr);
+        put<DT, SMT::XP, NP>(s.B[0], Q * SMT::LN, SMT::LN, ub);
+        put_x<DT, NP, PT, false>(s, buf, ux, 3);
         __syncthreads();
         if (AHEAD) ask(t + Q);
-        scale_x(s, buf, 3);
         if (threadIdx.x < 32) {
             chunk_steps(a, s, buf ^ 1, raw, tokens(t + Q), A, bias);
             raw_steps(a, t + 2 * Q, tokens(t + 2 * Q), h, raw);
         }
-        __syncthreads();
         const float g = s.G[buf][Q - 1];
         update_state(st, s, expf(g), 3);
         log_dec += g * 1.4426950408889634f;
@@ -322,6 +337,7 @@ __global__ void __launch_bounds__(THREADS) ssm_out_kernel(SsmArgs a) {
     constexpr bool AHEAD = NP <= 64;
     const float Dh = a.D ? a.D[h] : 0.f, A = a.A[h], bias = a.dt_bias ? a.dt_bias[h] : 0.f;
     for (int i = threadIdx.x; i < PT; i += THREADS) s.bad[i] = Q;
+    if (threadIdx.x == 0) s.any_bad = 0;
     float raw[2];
     uint4 ub[Piece<NP>::N], uc[Piece<NP>::N], ux[Piece<PT>::N];
     auto tokens = [&](int64_t t) { return (int)max((int64_t)0, min((int64_t)Q, u.t1 - t)); };
@@ -345,9 +361,9 @@ __global__ void __launch_bounds__(THREADS) ssm_out_kernel(SsmArgs a) {
         const bool last = t + Q >= u.t1;
         if (!AHEAD) ask(t);
         __syncthreads();
-        put<DT, XP, NP, false>(s.B[0], Q * LN, LN, ub, nullptr);
-        put<DT, XP, NP, false>(s.C[0], Q * LN, LN, uc, nullptr);
-        put<DT, XP, PT, true>(s.x[0], Q * LP, LP, ux, s.bad);
+        put<DT, XP, NP>(s.B[0], Q * LN, LN, ub);
+        put<DT, XP, NP>(s.C[0], Q * LN, LN, uc);
+        put_x<DT, NP, PT, true>(s, buf, ux, !last || a.ht ? pieces : 0);
         each_state<NP, PT>(st, [&](int p, int nn, float v) {
             const __nv_bfloat16 hi = __float2bfloat16_rn(v);
             s.S[0][p * LN + nn] = hi;
@@ -369,8 +385,6 @@ __global__ void __launch_bounds__(THREADS) ssm_out_kernel(SsmArgs a) {
                     if (a.z_pair) zr[j][k] = __ldg(reinterpret_cast<const uint32_t*>(src));
                     else zr[j][k] = __ldg(src) | (p + 1 < a.P ? (uint32_t)__ldg(src + 1) << 16 : 0u);
                 }
-        if (!last || a.ht) scale_x(s, buf, pieces);
-
         // rows 16 warp .. +15: what the state gives them, e^{G_i} C_i S^T
         const int m0 = 16 * warp;
         const float gi[2] = {s.G[buf][m0 + g], s.G[buf][m0 + g + 8]};
@@ -426,6 +440,7 @@ __global__ void __launch_bounds__(THREADS) ssm_out_kernel(SsmArgs a) {
                 }
         }
         // D x, gate, store
+        const bool odd = s.any_bad;
 #pragma unroll
         for (int j = 0; j < PT / 8; ++j)
 #pragma unroll
@@ -438,8 +453,10 @@ __global__ void __launch_bounds__(THREADS) ssm_out_kernel(SsmArgs a) {
                     xv.x += lo.x; xv.y += lo.y;
                 }
                 float2 v = make_float2(fmaf(Dh, xv.x, acc[j][2 * k]), fmaf(Dh, xv.y, acc[j][2 * k + 1]));
-                if (i >= s.bad[p]) v.x = __int_as_float(0x7fc00000);
-                if (i >= s.bad[p + 1]) v.y = __int_as_float(0x7fc00000);
+                if (odd) {
+                    if (i >= s.bad[p]) v.x = __int_as_float(0x7fc00000);
+                    if (i >= s.bad[p + 1]) v.y = __int_as_float(0x7fc00000);
+                }
                 if (a.z) {
                     const float2 z = DT == LAMPA_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&zr[j][k])) : unpack_bf16x2(zr[j][k]);
                     v.x *= z.x * sigmoidf_(z.x);
@@ -461,7 +478,7 @@ __global__ void __launch_bounds__(THREADS) ssm_out_kernel(SsmArgs a) {
         if (last && !(single && a.ht)) break;
         __syncthreads();
         update_state(st, s, expf(s.G[buf][Q - 1]), pieces);
-        each_state<NP, PT>(st, [&](int p, int, float& v) { if (s.bad[p] < Q) v = __int_as_float(0x7fc00000); });
+        if (odd) each_state<NP, PT>(st, [&](int p, int, float& v) { if (s.bad[p] < Q) v = __int_as_float(0x7fc00000); });
     }
     if (single && a.ht) {
         float* out = a.ht + ((int64_t)u.seq * a.H + h) * pn;
