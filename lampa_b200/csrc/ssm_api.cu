@@ -16,19 +16,21 @@ bool built(const lampa_ssm_desc* d) {
 }
 
 // The tcgen05 kernels take bf16 rows in pieces of 16 bytes, and their state is one operand tile.  Up to 128 tokens of few heads the
-// mma.sync form is one launch that ends with the state (37 tokens, 8 heads of 64 x 64: 13.1 us; tcgen05: 20.4 in three).
+// mma.sync form is one launch that ends with the state (37 tokens, 8 heads of 64 x 64: 10.8 us; tcgen05: 20.4 in three).
 bool umma_shape(const lampa_ssm_desc* d) {
     const bool few = d->T <= 2 * SSM_Q && (int64_t)d->B * d->H * ((d->P + 63) / 64) <= 2 * sm_count();
     return d->dtype == LAMPA_BF16 && d->P % 8 == 0 && d->N % 8 == 0 && d->N <= 128 && !few;
 }
 
-// Tokens per block.  mma.sync: enough blocks for eight CTAs to an SM, the last of every packed sequence aside where they are few (24 001 tokens in fp16, 6 heads of
-// 32 x 16: 68 us; with six and without that 80, with four 71, with two 98); tcgen05: for one CTA (of two heads) to an SM.
+// Tokens per block: enough blocks for eight CTAs to an SM in the mma.sync form (24 001 packed tokens in fp16, 6 heads of 32 x 16: with eight 68 us,
+// six 80, four 71, two 98, when these were compared), for one CTA (of two heads) to an SM in the tcgen05 form, where a second round of CTAs costs as much as the first.
+// Sequences of one length are cut into equally many blocks (four of 2 049 tokens, 8 pairs of heads: 49 us; by all tokens, 160 CTAs, 60); of a packed batch's, each may end in one that is not whole.
 int block_tokens(const lampa_ssm_desc* d, bool umma) {
     const int q = umma ? 128 : SSM_Q;
-    const int64_t n_tok = (int64_t)d->B * d->T, chunks = (n_tok + q - 1) / q, slabs = (d->P + 63) / 64;
-    const int64_t per = umma ? (int64_t)d->G * ((d->H / d->G + 1) / 2) * slabs : d->H * slabs;
-    const int64_t all = (umma ? 1 : 8) * (int64_t)sm_count() / per, want = std::max<int64_t>(1, umma ? all : std::max(all / 4, all - d->nseq));
+    const int64_t slabs = (d->P + 63) / 64, per = umma ? (int64_t)d->G * ((d->H / d->G + 1) / 2) * slabs : d->H * slabs;
+    const int64_t all = (umma ? 1 : 8) * (int64_t)sm_count() / per;
+    const int64_t chunks = ((int64_t)d->T + q - 1) / q;            // of a sequence, or of all of them
+    const int64_t want = std::max<int64_t>(1, d->nseq ? std::max(all / 4, all - d->nseq) : all / d->B);
     return (int)std::min<int64_t>(1 << 20, std::max<int64_t>(umma ? 1 : 2, (chunks + want - 1) / want)) * q;
 }
 
