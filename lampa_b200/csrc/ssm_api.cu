@@ -15,10 +15,10 @@ bool built(const lampa_ssm_desc* d) {
     return (d->dtype == LAMPA_BF16 || d->dtype == LAMPA_F16) && d->N <= 256 && d->H <= 65535 && d->P <= 65535;
 }
 
-// The tcgen05 kernels take bf16 rows in pieces of 16 bytes, and their state is one operand tile.  Up to 128 tokens of few heads the
-// mma.sync form is one launch that ends with the state (37 tokens, 8 heads of 64 x 64: 10.8 us; tcgen05: 20.4 in three).
+// The tcgen05 kernels take bf16 rows in pieces of 16 bytes, and their state is one operand tile.  One chunk of few heads is one launch
+// of the mma.sync form that ends with the state (64 tokens, 8 heads of 64 x 64: 11.0 us; tcgen05, in three launches: 17; 128 tokens: 18.2 and 16.6).
 bool umma_shape(const lampa_ssm_desc* d) {
-    const bool few = d->T <= 2 * SSM_Q && (int64_t)d->B * d->H * ((d->P + 63) / 64) <= 2 * sm_count();
+    const bool few = d->T <= SSM_Q && (int64_t)d->B * d->H * ((d->P + 63) / 64) <= 2 * sm_count();
     return d->dtype == LAMPA_BF16 && d->P % 8 == 0 && d->N % 8 == 0 && d->N <= 128 && !few;
 }
 
@@ -31,7 +31,7 @@ int block_tokens(const lampa_ssm_desc* d, bool umma) {
     const int64_t all = (umma ? 1 : 8) * (int64_t)sm_count() / per;
     const int64_t chunks = ((int64_t)d->T + q - 1) / q;            // of a sequence, or of all of them
     const int64_t want = std::max<int64_t>(1, d->nseq ? std::max(all / 4, all - d->nseq) : all / d->B);
-    return (int)std::min<int64_t>(1 << 20, std::max<int64_t>(umma ? 1 : 2, (chunks + want - 1) / want)) * q;
+    return (int)std::min<int64_t>(1 << 20, std::max<int64_t>(1, (chunks + want - 1) / want)) * q;
 }
 
 struct Plan { int bl, nb; int64_t units; bool blocks; size_t state_bytes, bytes; };
