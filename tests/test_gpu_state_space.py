@@ -237,16 +237,20 @@ def test_scan_offsets_on_the_device_are_checked(lb):
 def test_scan_waits_are_bounded(lb):
     """With no polls left every wait gives up: the call ends, says so, and the next one is right"""
     from lampa_b200 import _lib
-    a = scan_inputs(12, 1, 1000, 4, 64, 1, 128, BF, z=True, h0=True)
-    try:
-        _lib.lib().lampa_debug_set_poll_budget(0)
-        lb.state_space_scan(**a, output_final_state=True)
-        torch.cuda.synchronize()
-    finally:
-        _lib.lib().lampa_debug_set_poll_budget(1 << 22)
-    with pytest.raises(lb.LampaError):
+    for H, T in ((4, 1000), (48, 1500)):          # blocks of one chunk, and of several
+        a = scan_inputs(12, 1, T, H, 64, 1, 128, BF, z=True, h0=True)
+        want = lb.state_space_scan(**a, output_final_state=True)
+        try:
+            _lib.lib().lampa_debug_set_poll_budget(0)
+            lb.state_space_scan(**a, output_final_state=True)
+            torch.cuda.synchronize()
+        finally:
+            _lib.lib().lampa_debug_set_poll_budget(1 << 22)
+        with pytest.raises(lb.LampaError):
+            lb.check_status()
+        again = lb.state_space_scan(**a, output_final_state=True)
         lb.check_status()
-    check_scan(lb, a)
+        assert torch.equal(want[0], again[0]) and torch.equal(want[1], again[1])
 
 
 def test_scan_in_a_graph_and_on_another_stream(lb):
