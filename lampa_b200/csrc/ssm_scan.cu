@@ -13,8 +13,8 @@
 // A token whose x is not finite must not reach the rows in front of it through a zero of the mask (0 * NaN): such elements are taken
 // out of the tile, and from their row on the column is NaN, as the recurrence has it.
 //
-// What bounds it: instructions (24 001 packed tokens in fp16, 6 heads of 32 x 16, 62 us in all: output 34 us, issue slots 44 %, tensor pipe 10 %,
-// DRAM 5 %; states 18, pass 9), most of them spent on splitting fp16 into pieces, on decays and on the gate, in four warps a CTA whose phases
+// What bounds it: instructions (24 001 packed tokens in fp16, 6 heads of 32 x 16, 60 us in all: output 34 us, issue slots 44 %, tensor pipe 10 %,
+// DRAM 5 %; states 17, pass 9), most of them spent on splitting fp16 into pieces, on decays and on the gate, in four warps a CTA whose phases
 // follow one another.  With tiles and steps loaded just before their use 107 us, with the weighted pieces made from the tile in shared memory 68.  61 440 bf16 tokens, 16 heads of 64 x 128, take 1 120 us here and
 // 214 in the tcgen05 form.
 #include "profile.cuh"
@@ -32,12 +32,14 @@ template <int DT, int NP, int PT>
 struct Sm {
     static constexpr int XP = DT == LAMPA_F16 ? 2 : 1;                 // bf16 pieces of an input
     static constexpr int LN = NP + 8, LP = PT + 8;                     // row pitches: 16 bytes more than a power of two
+    static constexpr int STATE_BYTES = XP * Q * LN * 2 + 3 * Q * LP * 2 + 6 * Q * 4;     // up to and without C: all that ssm_state_kernel uses
     __nv_bfloat16 B[XP][Q * LN];
+    __nv_bfloat16 wx[3][Q * LP];                                       // d x e^{G_last - G}
+    float G[2][Q], d[2][Q], w[2][Q];                                   // by chunk parity
+    // (the output's alone)
     __nv_bfloat16 C[XP][Q * LN];
     __nv_bfloat16 S[XP][PT * LN];                                      // state as the right operand of C S^T
     __nv_bfloat16 x[XP][Q * LP];
-    __nv_bfloat16 wx[3][Q * LP];                                       // d x e^{G_last - G}
-    float G[2][Q], d[2][Q], w[2][Q];                                   // by chunk parity
     int bad[PT], any_bad;                                              // first row of the column that is not finite, or Q; whether there is one
 };
 
@@ -225,7 +227,7 @@ __global__ void __launch_bounds__(THREADS) ssm_state_kernel(SsmArgs a) {
     const int h = blockIdx.y, p0 = blockIdx.z * PT;
     if (!ssm_unit(a, blockIdx.x, u) || u.outside || u.single(a.bl)) return;
     using SMT = Sm<DT, NP, PT>;
-    constexpr bool AHEAD = NP <= 64;
+    constexpr bool AHEAD = NP <= 128;
     const int grp = h / (a.H / a.G);
     const float A = a.A[h], bias = a.dt_bias ? a.dt_bias[h] : 0.f;
     float st[StateMap<NP, PT>::CT][2][4] = {};
@@ -491,14 +493,16 @@ __global__ void __launch_bounds__(THREADS) ssm_out_kernel(SsmArgs a) {
 template <int DT, int NP, int PT>
 int launch_np(const SsmArgs& a, int units, bool blocks, cudaStream_t st) {
     static std::atomic<uint64_t> ready_s{0}, ready_o{0};
-    const int smem = (int)sizeof(Sm<DT, NP, PT>);
+    using SMT = Sm<DT, NP, PT>;
+    const int smem = (int)sizeof(Sm<DT, NP, PT>), smem_s = (int)SMT::STATE_BYTES;
     static_assert(sizeof(Sm<DT, NP, PT>) <= MAX_SMEM, "tiles fit");
+    static_assert(offsetof(SMT, C) == SMT::STATE_BYTES, "what the block kernel uses comes first");
     const dim3 grid(units, a.H, (a.P + PT - 1) / PT);
     if (blocks) {
-        if (!allow_smem(ready_s, ssm_state_kernel<DT, NP, PT>, smem)) return LAMPA_ERR_CUDA;
+        if (!allow_smem(ready_s, ssm_state_kernel<DT, NP, PT>, smem_s)) return LAMPA_ERR_CUDA;
         {
             ProfScope prof("ssm_state", st);
-            if (launch_chained(ssm_state_kernel<DT, NP, PT>, grid, dim3(THREADS), smem, st, a) != cudaSuccess) return LAMPA_ERR_CUDA;
+            if (launch_chained(ssm_state_kernel<DT, NP, PT>, grid, dim3(THREADS), smem_s, st, a) != cudaSuccess) return LAMPA_ERR_CUDA;
         }
     }
     if (blocks || (a.cu && a.ht)) {
