@@ -15,12 +15,10 @@ bool built(const lampa_ssm_desc* d) {
     return (d->dtype == LAMPA_BF16 || d->dtype == LAMPA_F16) && d->N <= 256 && d->H <= 65535 && d->P <= 65535;
 }
 
-// The tcgen05 kernels take bf16 rows in pieces of 16 bytes, and their state is one operand tile.  One chunk of few heads is one launch
-// of the mma.sync form that ends with the state (64 tokens, 8 heads of 64 x 64: 11.0 us; tcgen05, in three launches: 17; 128 tokens: 18.2 and 16.6).
-bool umma_shape(const lampa_ssm_desc* d) {
-    const bool few = d->T <= SSM_Q && (int64_t)d->B * d->H * ((d->P + 63) / 64) <= 2 * sm_count();
-    return d->dtype == LAMPA_BF16 && d->P % 8 == 0 && d->N % 8 == 0 && d->N <= 128 && !few;
-}
+// The tcgen05 kernels take bf16 rows in pieces of 16 bytes, and their state is one operand tile.  A single chunk is one launch of the mma.sync
+// form that ends with the state (64 tokens, 8 heads of 64 x 64: 11.0 us, tcgen05 in three launches 17; 256 such prompts: 89 and 150; 128 tokens:
+// 18.2 and 16.6).
+bool umma_shape(const lampa_ssm_desc* d) { return d->dtype == LAMPA_BF16 && d->P % 8 == 0 && d->N % 8 == 0 && d->N <= 128 && d->T > SSM_Q; }
 
 // Tokens per block: enough blocks for eight CTAs to an SM in the mma.sync form (24 001 packed tokens in fp16, 6 heads of 32 x 16: with eight 68 us,
 // six 80, four 71, two 98, when these were compared), for one CTA (of two heads) to an SM in the tcgen05 form, where a second round of CTAs costs as much as the first.
