@@ -15,7 +15,7 @@ struct SsmArgs {
     const int64_t* cu;
     void* y; float* ht;
     float* blk;                       // [units][H][P][N]: end states of blocks that begin empty, then the states that enter them
-    float* blk_dec;                   // [units][H]: log2 of a block's decay
+    float* blk_dec;                   // [units][H]: logarithm of a block's decay
     int32_t* status;
     int64_t x_tok, x_head, z_tok, z_head, b_tok, b_grp, c_tok, c_grp, dt_tok;   // distances in elements
     int64_t n_tok, T;                 // rows in all; tokens per sequence without cu
@@ -77,6 +77,18 @@ inline int64_t ssm_units(int64_t n_tok, int nseq, int nb, int bl, bool packed) {
 // log(1 + e^x) to fp32 rounding: the states are kept to a few parts in 10^7, and softplusf_ is good to 2e-7 of 1
 __device__ __forceinline__ float ssm_step_size(float v, int softplus) {
     return softplus ? fmaxf(v, 0.f) + log1pf(expf(-fabsf(v))) : v;
+}
+
+// Sums of exponents g = A d, of which the kernels need differences inside a chunk.  Counted from the chunk's start as one float, a token with a large
+// step leaves the sum large for the rest of its chunk and rounds the small steps behind it to 2^-24 of that.  So a chunk is cut into blocks of a few
+// tokens: between blocks only sums of one sign are added up (from a token to its block's end, of whole blocks, from a block's start to a
+// token), each with an error of its own size; inside a block differences of sums from its start are taken, in two parts: whole numbers, which add up exactly
+// (a g below SSM_CUT is cut: its exponential is zero all the same), and the rest, half at most in size.  (NaN stays NaN.)
+constexpr float SSM_CUT = -128.f;
+struct SsmExp { float whole, rest; };
+__device__ __forceinline__ SsmExp ssm_split(float g) {
+    const float c = g < SSM_CUT ? SSM_CUT : g, w = rintf(c);
+    return {w, c - w};
 }
 
 int launch_ssm_pass(const SsmArgs& a, cudaStream_t st);

@@ -32,14 +32,16 @@ template <int DT, int NP, int PT>
 struct Sm {
     static constexpr int XP = DT == LAMPA_F16 ? 2 : 1;                 // bf16 pieces of an input
     static constexpr int LN = NP + 8, LP = PT + 8;                     // row pitches: 16 bytes more than a power of two
-    static constexpr int STATE_BYTES = XP * Q * LN * 2 + 3 * Q * LP * 2 + 6 * Q * 4;     // up to and without C: all that ssm_state_kernel uses
+    static constexpr int STATE_BYTES = XP * Q * LN * 2 + 3 * Q * LP * 2 + 2 * Q * 4 + 2 * 4 * 4;     // up to and without C: all that ssm_state_kernel uses
     __nv_bfloat16 B[XP][Q * LN];
     __nv_bfloat16 wx[3][Q * LP];                                       // d x e^{G_last - G}
-    float G[2][Q], d[2][Q], w[2][Q];                                   // by chunk parity
+    float w[2][Q], sum[2][4];                                          // by chunk parity; sums of A d of 16 tokens each
     // (the output's alone)
     __nv_bfloat16 C[XP][Q * LN];
     __nv_bfloat16 S[XP][PT * LN];                                      // state as the right operand of C S^T
     __nv_bfloat16 x[XP][Q * LP];
+    SsmExp G[2][Q];                                                    // sums of A d from the first of the token's 16 on
+    float d[2][Q], cf[2][Q];                                           // cf = d e^{what follows in the token's 16}
     int bad[PT], any_bad;                                              // first row of the column that is not finite, or Q; whether there is one
 };
 
@@ -129,9 +131,9 @@ __device__ __forceinline__ void put_x(Sm<DT, NP, PT>& s, int buf, uint4 (&u)[Pie
     if (KEEP) put<DT, S::XP, PT>(s.x[0], Q * S::LP, S::LP, u);
 }
 
-// d, G and w = d e^{G_last - G} of a chunk's n tokens (tokens beyond them have d = 0), by the first warp, two tokens to a lane: raw steps a
-// chunk ahead, the rest while the other warps, which have more scores to work on, are busy.  The exponent of w is summed from the end of
-// the chunk: it then carries an error of its own size, not of G's.
+// d and w = d e^{G_last - G} of a chunk's n tokens (tokens beyond them have d = 0), and FULL: what the decays between two of them are made
+// from, by the first warp, two tokens to a lane: raw steps a chunk ahead, the rest while the other warps, which have more scores to work on,
+// are busy.  Every exponent is a sum of what lies between its two tokens, or exact but for its rest (SsmExp), so that its error is one of its own size, not of G's.
 __device__ __forceinline__ void raw_steps(const SsmArgs& a, int64_t t0, int n, int h, float (&raw)[2]) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -139,7 +141,7 @@ __device__ __forceinline__ void raw_steps(const SsmArgs& a, int64_t t0, int n, i
         raw[k] = i < n ? load_as_float(a.dt, (size_t)((t0 + i) * a.dt_tok + h), a.dt_dt) : 0.f;
     }
 }
-template <typename SM>
+template <bool FULL, typename SM>
 __device__ __forceinline__ void chunk_steps(const SsmArgs& a, SM& s, int buf, const float (&raw)[2], int n, float A, float bias) {
     const int l = threadIdx.x & 31;
     float d[2], g[2];
@@ -148,20 +150,41 @@ __device__ __forceinline__ void chunk_steps(const SsmArgs& a, SM& s, int buf, co
         d[k] = 2 * l + k < n ? ssm_step_size(raw[k] + bias, a.softplus) : 0.f;
         g[k] = 2 * l + k < n ? d[k] * A : 0.f;
     }
-    float up = g[0] + g[1], down = up;
+    float down = g[0] + g[1];                      // to the end of its 16 tokens, which eight lanes hold
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const float u = __shfl_up_sync(0xffffffffu, up, o), v = __shfl_down_sync(0xffffffffu, down, o);
-        if (l >= o) up += u;
-        if (l + o < 32) down += v;
+    for (int o = 1; o < 8; o <<= 1) {
+        const float v = __shfl_down_sync(0xffffffffu, down, o, 8);
+        if ((l & 7) + o < 8) down += v;
     }
-    const float before = __shfl_up_sync(0xffffffffu, up, 1), after = __shfl_down_sync(0xffffffffu, down, 1);
-    const float b = l ? before : 0.f, e = l < 31 ? after : 0.f;
-    s.d[buf][2 * l] = d[0]; s.d[buf][2 * l + 1] = d[1];
-    s.G[buf][2 * l] = b + g[0]; s.G[buf][2 * l + 1] = up;
+    const float next = __shfl_down_sync(0xffffffffu, down, 1, 8), after = (l & 7) < 7 ? next : 0.f;
+    float sum[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) sum[b] = __shfl_sync(0xffffffffu, down, 8 * b);
+    float e = 0.f;                                 // of the 16-token blocks behind this one
+#pragma unroll
+    for (int b = 3; b > 0; --b) e += l < 8 * b ? sum[b] : 0.f;
+    e += after;
     s.w[buf][2 * l] = d[0] * expf(e + g[1]);
     s.w[buf][2 * l + 1] = d[1] * expf(e);
+    if (l < 4) s.sum[buf][l] = l < 2 ? l == 0 ? sum[0] : sum[1] : l == 2 ? sum[2] : sum[3];
+    if constexpr (FULL) {
+        const SsmExp g0 = ssm_split(g[0]), g1 = ssm_split(g[1]);
+        SsmExp up = {g0.whole + g1.whole, g0.rest + g1.rest};
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+            const float u = __shfl_up_sync(0xffffffffu, up.whole, o, 8), r = __shfl_up_sync(0xffffffffu, up.rest, o, 8);
+            if ((l & 7) >= o) { up.whole += u; up.rest += r; }
+        }
+        const float bw = __shfl_up_sync(0xffffffffu, up.whole, 1, 8), br = __shfl_up_sync(0xffffffffu, up.rest, 1, 8);
+        s.G[buf][2 * l] = {((l & 7) ? bw : 0.f) + g0.whole, ((l & 7) ? br : 0.f) + g0.rest};
+        s.G[buf][2 * l + 1] = up;
+        s.d[buf][2 * l] = d[0]; s.d[buf][2 * l + 1] = d[1];
+        s.cf[buf][2 * l] = d[0] * __expf(after + g[1]);
+        s.cf[buf][2 * l + 1] = d[1] * __expf(after);
+    }
 }
+template <typename SM>
+__device__ __forceinline__ float chunk_sum(const SM& s, int buf) { return (s.sum[buf][0] + s.sum[buf][1]) + (s.sum[buf][2] + s.sum[buf][3]); }
 
 // The state of a CTA: PT x NP, warp w holds rows 16 (w % RS) .. +15 and columns of 16 (cg + CG i)
 template <int NP, int PT>
@@ -241,7 +264,7 @@ __global__ void __launch_bounds__(THREADS) ssm_state_kernel(SsmArgs a) {
     if (threadIdx.x < 32) raw_steps(a, u.t0, tokens(u.t0), h, raw);
     if (AHEAD) ask(u.t0);
     if (threadIdx.x < 32) {
-        chunk_steps(a, s, 0, raw, tokens(u.t0), A, bias);
+        chunk_steps<false>(a, s, 0, raw, tokens(u.t0), A, bias);
         raw_steps(a, u.t0 + Q, tokens(u.t0 + Q), h, raw);
     }
     int buf = 0;
@@ -253,12 +276,12 @@ __global__ void __launch_bounds__(THREADS) ssm_state_kernel(SsmArgs a) {
         __syncthreads();
         if (AHEAD) ask(t + Q);
         if (threadIdx.x < 32) {
-            chunk_steps(a, s, buf ^ 1, raw, tokens(t + Q), A, bias);
+            chunk_steps<false>(a, s, buf ^ 1, raw, tokens(t + Q), A, bias);
             raw_steps(a, t + 2 * Q, tokens(t + 2 * Q), h, raw);
         }
-        const float g = s.G[buf][Q - 1];
+        const float g = chunk_sum(s, buf);
         update_state(st, s, expf(g), 3);
-        log_dec += g * 1.4426950408889634f;
+        log_dec += g;
     }
     float* out = a.blk + ((int64_t)blockIdx.x * a.H + h) * a.P * a.N;
     each_state<NP, PT>(st, [&](int p, int n, float v) {
@@ -304,7 +327,7 @@ __global__ void __launch_bounds__(256) ssm_pass_kernel(SsmArgs a) {
             for (int k = 0; k < AHEAD; ++k)
                 if (b + k < nb) {
                     *reinterpret_cast<Vec*>(p + (b + k) * step) = s;
-                    const float x = exp2f(d[k]);
+                    const float x = expf(d[k]);
 #pragma unroll
                     for (int i = 0; i < V; ++i) s.v[i] = fmaf(x, s.v[i], part[k].v[i]);
                 }
@@ -314,7 +337,7 @@ __global__ void __launch_bounds__(256) ssm_pass_kernel(SsmArgs a) {
 }
 
 template <int DT, int NP, int PT>
-__global__ void __launch_bounds__(THREADS) ssm_out_kernel(SsmArgs a) {
+__global__ void __launch_bounds__(THREADS, NP * PT <= 512 && (DT == LAMPA_BF16 || NP == 16) ? 4 : 0) ssm_out_kernel(SsmArgs a) {     // (four: 128 registers, where that spills nothing)
     using SMT = Sm<DT, NP, PT>;
     constexpr int XP = SMT::XP, LN = SMT::LN, LP = SMT::LP;
     if (chain_wait()) return;
@@ -353,7 +376,7 @@ __global__ void __launch_bounds__(THREADS) ssm_out_kernel(SsmArgs a) {
     float st[StateMap<NP, PT>::CT][2][4];
     each_state<NP, PT>(st, [&](int p, int n, float& v) { v = enter && p0 + p < a.P && n < a.N ? enter[(int64_t)(p0 + p) * a.N + n] : 0.f; });
     if (warp == 0) {
-        chunk_steps(a, s, 0, raw, tokens(u.t0), A, bias);
+        chunk_steps<true>(a, s, 0, raw, tokens(u.t0), A, bias);
         raw_steps(a, u.t0 + Q, tokens(u.t0 + Q), h, raw);
     }
 
@@ -389,7 +412,8 @@ __global__ void __launch_bounds__(THREADS) ssm_out_kernel(SsmArgs a) {
                 }
         // rows 16 warp .. +15: what the state gives them, e^{G_i} C_i S^T
         const int m0 = 16 * warp;
-        const float gi[2] = {s.G[buf][m0 + g], s.G[buf][m0 + g + 8]};
+        const SsmExp gi[2] = {s.G[buf][m0 + g], s.G[buf][m0 + g + 8]};
+        float from[2] = {gi[0].whole + gi[0].rest, gi[1].whole + gi[1].rest};      // sums from the start of the 16 columns behind the tile's
         float acc[PT / 8][4] = {};
 #pragma unroll
         for (int cp = XP - 1; cp >= 0; --cp)
@@ -397,19 +421,44 @@ __global__ void __launch_bounds__(THREADS) ssm_out_kernel(SsmArgs a) {
             for (int sp = XP - 1 - cp; sp >= 0; --sp)
                 warp_gemm<PT / 8, NP, false, false>(acc, s.C[cp], LN, m0, s.S[sp], LN, 0, lane);
         {
-            const float e0 = __expf(gi[0]), e1 = __expf(gi[1]);
+            float before = 0.f;
+#pragma unroll
+            for (int b = 0; b < 3; ++b) before += b < warp ? s.sum[buf][b] : 0.f;
+            const float e0 = __expf(before + from[0]), e1 = __expf(before + from[1]);
 #pragma unroll
             for (int j = 0; j < PT / 8; ++j) { acc[j][0] *= e0; acc[j][1] *= e0; acc[j][2] *= e1; acc[j][3] *= e1; }
         }
-        // and the tokens of the chunk up to their own: 16 columns of scores at a time
+        // and the tokens of the chunk up to their own: 16 columns of scores at a time, their own 16 first.  In front of those e^{G_i - G_j} is
+        // a row's factor to the 16 columns' end and a column's from there
 #pragma unroll 1
-        for (int j0 = 0; j0 <= m0; j0 += 16) {
+        for (int j0 = m0; j0 >= 0; j0 -= 16) {
             float sc[2][4] = {};
 #pragma unroll
             for (int cp = XP - 1; cp >= 0; --cp)
 #pragma unroll
                 for (int bp = XP - 1 - cp; bp >= 0; --bp)
                     warp_gemm<2, NP, false, false>(sc, s.C[cp], LN, m0, s.B[bp], LN, j0, lane);
+            float dec[2][4];
+            if (j0 == m0) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const int j = m0 + 8 * c + t2 + k;
+                        const SsmExp gj = s.G[buf][j];
+                        const float d = s.d[buf][j];
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) dec[c][2 * r + k] = __expf((gi[r].whole - gj.whole) + (gi[r].rest - gj.rest)) * d;
+                    }
+            } else {
+                const float r0 = __expf(from[0]), r1 = __expf(from[1]), sum = s.sum[buf][j0 / 16];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float2 cf = *reinterpret_cast<const float2*>(&s.cf[buf][j0 + 8 * c + t2]);
+                    dec[c][0] = r0 * cf.x; dec[c][1] = r0 * cf.y; dec[c][2] = r1 * cf.x; dec[c][3] = r1 * cf.y;
+                }
+                from[0] += sum; from[1] += sum;
+            }
             uint32_t pa[XP][4];
 #pragma unroll
             for (int c = 0; c < 2; ++c)
@@ -417,10 +466,8 @@ __global__ void __launch_bounds__(THREADS) ssm_out_kernel(SsmArgs a) {
                 for (int r = 0; r < 2; ++r) {
                     float v[2];
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const int i = m0 + g + 8 * r, j = j0 + 8 * c + t2 + k;
-                        v[k] = j <= i ? sc[c][2 * r + k] * __expf(gi[r] - s.G[buf][j]) * s.d[buf][j] : 0.f;
-                    }
+                    for (int k = 0; k < 2; ++k)
+                        v[k] = j0 < m0 || 8 * c + t2 + k <= g + 8 * r ? sc[c][2 * r + k] * dec[c][2 * r + k] : 0.f;
                     const uint32_t w = pack_bf16x2(v[0], v[1]);
                     pa[0][2 * c + r] = w;
                     if (XP > 1) {
@@ -474,12 +521,12 @@ __global__ void __launch_bounds__(THREADS) ssm_out_kernel(SsmArgs a) {
                 }
             }
         if (warp == 0 && !last) {
-            chunk_steps(a, s, buf ^ 1, raw, tokens(t + Q), A, bias);
+            chunk_steps<true>(a, s, buf ^ 1, raw, tokens(t + Q), A, bias);
             raw_steps(a, t + 2 * Q, tokens(t + 2 * Q), h, raw);
         }
         if (last && !(single && a.ht)) break;
         __syncthreads();
-        update_state(st, s, expf(s.G[buf][Q - 1]), pieces);
+        update_state(st, s, expf(chunk_sum(s, buf)), pieces);
         if (odd) each_state<NP, PT>(st, [&](int p, int, float& v) { if (s.bad[p] < Q) v = __int_as_float(0x7fc00000); });
     }
     if (single && a.ht) {

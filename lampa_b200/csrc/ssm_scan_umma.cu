@@ -52,18 +52,21 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
                  :: "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(t), "r"(smem_u32(bar)) : "memory");
 }
 
-// Per head and chunk, by token: G (log2), d, d e^{G_end(32-block) - G}, d e^{G_last - G}
-struct Tab { float G[UQ], d[UQ], cf[UQ], w[UQ]; };
+// Per head and chunk, by token: G (log2, from the start of its 32 tokens on), d, d e^{what follows in its 32}, d e^{G_last - G}; between[q][b]: log2
+// of the decay of the 32-token blocks behind b and in front of q, [q][q] of all in front of q
+struct Tab { float G[UQ], d[UQ], cf[UQ], w[UQ], between[4][4]; };
 
-// One warp, four tokens to a lane, one head.  The steps are asked for a chunk ahead (raw); tokens from n on have d = 0.  Returns log2 of the
-// chunk's decay.  The exponent of w is summed from the chunk's end, so that its error is one of its own size.
+// One warp, four tokens to a lane, one head.  The steps are asked for a chunk ahead (raw); tokens from n on have d = 0.  Returns the logarithm of the
+// chunk's decay.  Every exponent is a sum of what lies between its two tokens, so that its error is one of its own size.  Inside 32 tokens
+// differences of G are taken, which is a sum of exact whole numbers and small rests (SsmExp), 32 x 128 at most and rounded once: a decay there is good to
+// 2 x 2^-13 ln 2 < 2^-12, a sixteenth of a step of the bf16 that it becomes.  What lies between blocks, and w, has no such limit.
 struct Steps {
-    float A2, bias;
+    float A, bias;
     int h;
     bool has;
     uint32_t raw[4];
     __device__ __forceinline__ Steps(const SsmArgs& a, int h0, int x, bool there) : h(there ? h0 + x : h0), has(there) {
-        A2 = a.A[h] * LOG2E;
+        A = a.A[h];
         bias = a.dt_bias ? a.dt_bias[h] : 0.f;
     }
     __device__ __forceinline__ void ask(const SsmArgs& a, int64_t t, int n) {      // n <= 0: there is no such chunk
@@ -77,36 +80,58 @@ struct Steps {
     template <bool FULL>
     __device__ __forceinline__ float make(const SsmArgs& a, float* ws, Tab* s, int n) const {
         const int l = threadIdx.x & 31;
-        float d[4], g[4], up = 0.f;
+        float d[4], g[4], down = 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const bool in = 4 * l + k < n && has;
             d[k] = in ? ssm_step_size(load_as_float(&raw[k], 0, a.dt_dt) + bias, a.softplus) : 0.f;
-            g[k] = in ? d[k] * A2 : 0.f;
-            up += g[k];
+            g[k] = in ? d[k] * A : 0.f;
+            down += g[k];
         }
-        float down = up;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const float u = __shfl_up_sync(0xffffffffu, up, o), v = __shfl_down_sync(0xffffffffu, down, o);
-            if (l >= o) up += u;
-            if (l + o < 32) down += v;
+        for (int o = 1; o < 8; o <<= 1) {          // to the end of its 32 tokens, which eight lanes hold
+            const float v = __shfl_down_sync(0xffffffffu, down, o, 8);
+            if ((l & 7) + o < 8) down += v;
         }
-        const float before = __shfl_up_sync(0xffffffffu, up, 1), after = __shfl_down_sync(0xffffffffu, down, 1);
-        float e = l < 31 ? after : 0.f, w[4];
+        const float next = __shfl_down_sync(0xffffffffu, down, 1, 8), after = (l & 7) < 7 ? next : 0.f;
+        float sum[4], e = 0.f, w[4];
 #pragma unroll
-        for (int k = 3; k >= 0; --k) { w[k] = d[k] * exp2f(e); e += g[k]; }
+        for (int b = 0; b < 4; ++b) sum[b] = __shfl_sync(0xffffffffu, down, 8 * b);
+#pragma unroll
+        for (int b = 3; b > 0; --b) e += l < 8 * b ? sum[b] : 0.f;
+        e += after;
+#pragma unroll
+        for (int k = 3; k >= 0; --k) { w[k] = d[k] * expf(e); e += g[k]; }
         *reinterpret_cast<float4*>(ws + 4 * l) = make_float4(w[0], w[1], w[2], w[3]);
         if (FULL) {
-            float G[4], b = l ? before : 0.f;
+            SsmExp G[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) { b += g[k]; G[k] = b; }
-            const float end = __shfl_sync(0xffffffffu, G[3], l | 7);
-            *reinterpret_cast<float4*>(&s->G[4 * l]) = make_float4(G[0], G[1], G[2], G[3]);
+            for (int k = 0; k < 4; ++k) {
+                const SsmExp x = ssm_split(g[k] * LOG2E);
+                G[k] = k ? SsmExp{G[k - 1].whole + x.whole, G[k - 1].rest + x.rest} : x;
+            }
+            SsmExp up = G[3];
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) {
+                const float u = __shfl_up_sync(0xffffffffu, up.whole, o, 8), r = __shfl_up_sync(0xffffffffu, up.rest, o, 8);
+                if ((l & 7) >= o) { up.whole += u; up.rest += r; }
+            }
+            const float pw = __shfl_up_sync(0xffffffffu, up.whole, 1, 8), pr = __shfl_up_sync(0xffffffffu, up.rest, 1, 8);
+            const SsmExp p = {(l & 7) ? pw : 0.f, (l & 7) ? pr : 0.f};
+            float cf[4], f = after;
+#pragma unroll
+            for (int k = 3; k >= 0; --k) { cf[k] = d[k] * ex2(f * LOG2E); f += g[k]; }
+            *reinterpret_cast<float4*>(&s->G[4 * l]) = make_float4((p.whole + G[0].whole) + (p.rest + G[0].rest), (p.whole + G[1].whole) + (p.rest + G[1].rest),
+                                                                   (p.whole + G[2].whole) + (p.rest + G[2].rest), (p.whole + G[3].whole) + (p.rest + G[3].rest));
             *reinterpret_cast<float4*>(&s->d[4 * l]) = make_float4(d[0], d[1], d[2], d[3]);
-            *reinterpret_cast<float4*>(&s->cf[4 * l]) = make_float4(d[0] * ex2(end - G[0]), d[1] * ex2(end - G[1]), d[2] * ex2(end - G[2]), d[3] * ex2(end - G[3]));
+            *reinterpret_cast<float4*>(&s->cf[4 * l]) = make_float4(cf[0], cf[1], cf[2], cf[3]);
+            float t = 0.f;
+            const int q = (l >> 2) & 3, b = l & 3;
+#pragma unroll
+            for (int m = 0; m < 3; ++m) t += m < q && (b == q || m > b) ? sum[m] : 0.f;
+            if (l < 16) s->between[q][b] = t * LOG2E;
         }
-        return __shfl_sync(0xffffffffu, up, 31);
+        return (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
 };
 
@@ -272,7 +297,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_state_umma_kernel(SsmArgs a, c
         p.ask(a, u.t0, rows(0));
         for (int c = 0; c < chunks; ++c) {
             const float g = p.make<false>(a, s.w[c & 1][x], nullptr, rows(c));
-            if (lane == 0) s.tot[c & 3][x] = exp2f(g);
+            if (lane == 0) s.tot[c & 3][x] = expf(g);
             log_dec += g;
             p.ask(a, u.t0 + (int64_t)(c + 1) * UQ, rows(c + 1));
             nb_sync<CS>(A_NEXT);
@@ -576,7 +601,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a, con
         p.ask(a, u.t0, rows(0));
         for (int c = 0; c < chunks; ++c) {
             const float g = p.make<true>(a, s.tab[c & 1][x].w, &s.tab[c & 1][x], rows(c));
-            if (lane == 0) s.tot[c & 1][x] = exp2f(g);
+            if (lane == 0) s.tot[c & 1][x] = expf(g);
             p.ask(a, u.t0 + (int64_t)(c + 1) * UQ, rows(c + 1));
             __syncwarp();
             nb_arrive<CS>(C_DS);                  // the states that enter chunk c may be decayed for what it adds
@@ -692,7 +717,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a, con
                 if (b < q) tmem_ld16_issue(nx, tl + TM_G + 32 * (b + 1) + j0);
                 uint32_t o[8];
                 if (b < q) {
-                    const F2 r = f2(ex2(Gi - t.G[32 * b + 31]));
+                    const F2 r = f2(ex2(Gi + t.between[q][b]));
 #pragma unroll
                     for (int j = 0; j < 16; j += 4) {
                         const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(&t.cf[32 * b + j0 + j]);
@@ -734,7 +759,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a, con
         nb_sync<CC>(C_Y);
         tc_fence_after();
         {
-            const F2 r = f2(ex2(Gi));
+            const F2 r = f2(ex2(Gi + t.between[q][q]));
             float yv[2][16];
             tmem_ld16_issue(yv[0], tl + TM_Y + 64 * hd + 32 * half);
             tmem_ld16_issue(yv[1], tl + TM_Y + 64 * hd + 32 * half + 16);

@@ -1,0 +1,61 @@
+"""The state space operators where a call is allowed but out of the ordinary, against the recurrence in 64 bits with the bounds of ssm_oracle.py."""
+import pytest
+import torch
+
+from tests.test_gpu_state_space import BF, F32, FP, check_scan, lb, scan_inputs  # noqa: F401  (lb is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _checked_by_the_tests(monkeypatch):
+    monkeypatch.setenv("LAMPA_B200_CHECK", "0")
+
+
+@pytest.fixture(params=["tcgen05", "mma.sync"])
+def form(request, lb):  # noqa: F811
+    from lampa_b200 import _lib
+    _lib.lib().lampa_debug_force_mma_sync(int(request.param == "mma.sync"))
+    yield request.param
+    _lib.lib().lampa_debug_force_mma_sync(0)
+
+
+# ---- scan: large steps among small ones --------------------------------------------------------------
+RESETS = {"sixth": [5], "some": [5, 70, 71, 127, 128, 200, 263], "seventh": list(range(0, 300, 7)), "second": list(range(1, 300, 2))}
+
+
+def reset_inputs(dtype, large, where, softplus, own, seed=21):
+    """Steps of 0.001 to 0.1 with `large` at some tokens, A = -16 and -1; own: these tokens add to the state, else their x is zero"""
+    a = scan_inputs(seed, 1, 300, 2, 64, 1, 64, dtype, z=True, h0=True, dt_dtype=F32)
+    a["A"] = torch.tensor([-16.0, -1.0], device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    d = 0.001 + 0.099 * torch.rand(1, 300, 2, generator=gen, device="cuda")
+    dt = torch.log(torch.expm1(d)) if softplus else d
+    dt[:, RESETS[where]] = large
+    a.update(dt=dt, dt_bias=None)
+    if not own:
+        x = a["x"].clone()
+        x[:, RESETS[where]] = 0
+        a["x"] = x
+    return a
+
+
+@pytest.mark.parametrize("softplus", [False, True])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("large", [6.0, 1e3, 1e4, 1e6, 1e30])
+@pytest.mark.parametrize("where", list(RESETS))
+def test_scan_small_steps_behind_a_large_one(lb, form, dtype, large, where, softplus):  # noqa: F811
+    """A large step resets the state; the tokens behind it in its chunk are as exact as any"""
+    if dtype == FP and form == "tcgen05":
+        pytest.skip("fp16 has the mma.sync form only")
+    for own in (False, True):
+        check_scan(lb, reset_inputs(dtype, large, where, softplus, own), softplus=softplus)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_scan_decay_beyond_the_largest_float(lb, form, dtype):  # noqa: F811
+    """A d below the lowest finite float is a decay of zero, also for the tokens behind it"""
+    a = reset_inputs(dtype, 1e35, "some", False, False)
+    a["A"] = torch.tensor([-1e4, -2.0], device="cuda")
+    a["dt"][..., 0] = torch.where(a["dt"][..., 0] < 1, a["dt"][..., 0] * 1e-3, a["dt"][..., 0])
+    check_scan(lb, a, softplus=False)
