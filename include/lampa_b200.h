@@ -523,12 +523,17 @@ int lampa_profile_read(char* names, size_t names_cap, float* total_ms, int32_t* 
 
 /*
  * Test hook (no counterpart in the reference): number of polls after which a device-side wait of
- * the gated-delta and model kernels gives up (default and maximum 2^22).  A test sets it to 0 to see the
+ * the gated-delta, model and state space kernels gives up (default and maximum 2^22).  A test sets it to 0 to see the
  * give-up path without anything hanging: the kernels then return at once, results are undefined
  * and LAMPA_ERR_TIMEOUT is in the status word; copies and MMAs already in flight are still waited
  * for with the full budget before a CTA exits.  Process-wide; not for concurrent use.
  */
 int lampa_debug_set_poll_budget(int polls);
+/*
+ * Test hook (no counterpart in the reference): the same for one of two warps that wait in the tcgen05 output pass of lampa_ssm_scan, the
+ * one that issues its products (lampa_debug_set_poll_budget sets both): a test sees one of them give up while the other does not.
+ */
+int lampa_debug_set_product_poll_budget(int polls);
 /*
  * Test hook (no counterpart in the reference): on = 1 routes the K = V = 64 gated-delta calls that follow to the
  * mma.sync kernels instead of the tcgen05 ones (what LAMPA_B200_NO_UMMA=1 does for a whole process), on = 0 back;

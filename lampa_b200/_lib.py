@@ -51,7 +51,7 @@ EXPORTS = ["lampa_version", "lampa_error_string", "lampa_gdn_workspace_bytes", "
            "lampa_ssm_workspace_bytes", "lampa_ssm_scan", "lampa_ssm_step", "lampa_short_conv_resume", "lampa_block_norm",
            "lampa_hgdn_fwd_again", "lampa_model_encode", "lampa_model_project", "lampa_model_update", "lampa_model_head",
            "lampa_repeat_segments", "lampa_profile_enable",
-           "lampa_profile_read", "lampa_debug_set_poll_budget", "lampa_debug_set_tick_buffer",
+           "lampa_profile_read", "lampa_debug_set_poll_budget", "lampa_debug_set_product_poll_budget", "lampa_debug_set_tick_buffer",
            "lampa_debug_force_mma_sync"]
 
 
@@ -108,6 +108,7 @@ def lib() -> ctypes.CDLL:
         L.lampa_repeat_segments.argtypes = [vp, i32, i32, i64, vp, vp]
         L.lampa_profile_enable.argtypes = [ctypes.c_int]
         L.lampa_debug_set_poll_budget.argtypes = [ctypes.c_int]
+        L.lampa_debug_set_product_poll_budget.argtypes = [ctypes.c_int]
         L.lampa_debug_force_mma_sync.argtypes = [ctypes.c_int]
         L.lampa_debug_set_tick_buffer.argtypes = [vp, ctypes.c_int]
         L.lampa_profile_read.argtypes = [ctypes.c_char_p, sz, ctypes.POINTER(ctypes.c_float),

@@ -155,6 +155,7 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 constexpr int MBAR_POLLS = 1 << 22;
 bool umma_enabled();               // false on the mma.sync twins (lampa_debug_force_mma_sync, LAMPA_B200_NO_UMMA=1)
 int poll_budget();                 // of the launches that follow (host): MBAR_POLLS unless lampa_debug_set_poll_budget lowered it
+int poll_budget_products();        // the same, where lampa_debug_set_product_poll_budget has its own
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, bool& dead, int32_t* status, int where, int budget) {
     if (dead) return false;
     for (int i = 0; i < budget; ++i)

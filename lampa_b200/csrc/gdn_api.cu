@@ -8,6 +8,8 @@ using namespace lampa;
 namespace lampa {
 static int g_poll_budget = MBAR_POLLS;
 int poll_budget() { return g_poll_budget; }
+static int g_poll_budget_products = MBAR_POLLS;
+int poll_budget_products() { return g_poll_budget_products; }
 static int g_force_mma_sync = 0;  // see lampa_debug_force_mma_sync
 bool umma_enabled() {
     static const bool off = [] { const char* e = getenv("LAMPA_B200_NO_UMMA"); return e && e[0] == '1'; }();
@@ -188,7 +190,13 @@ extern "C" int lampa_debug_force_mma_sync(int on) {
 
 extern "C" int lampa_debug_set_poll_budget(int polls) {
     if (polls < 0) return LAMPA_ERR_ARG;
-    g_poll_budget = polls > MBAR_POLLS ? MBAR_POLLS : polls;
+    g_poll_budget = g_poll_budget_products = polls > MBAR_POLLS ? MBAR_POLLS : polls;
+    return LAMPA_OK;
+}
+
+extern "C" int lampa_debug_set_product_poll_budget(int polls) {
+    if (polls < 0) return LAMPA_ERR_ARG;
+    g_poll_budget_products = polls > MBAR_POLLS ? MBAR_POLLS : polls;
     return LAMPA_OK;
 }
 

@@ -27,6 +27,7 @@ struct SsmArgs {
     int z_pair, y_pair;               // two neighbours of z, or y, are one aligned word
     int whole;                        // the block kernel also has the states of sequences of one block (tcgen05 form)
     int poll_budget;
+    int poll_budget_products;         // of the warp that issues the output pass's products (tcgen05 form)
 };
 
 // A block of tokens that one CTA walks through.  Packed sequences need no table: block b of sequence s has the number

@@ -92,5 +92,6 @@ extern "C" int lampa_ssm_scan(const lampa_ssm_desc* d, const void* x, int64_t x_
     a.y_pair = d->P % 2 == 0 && ((uintptr_t)y & 3) == 0;
     a.whole = umma;
     a.poll_budget = poll_budget();
+    a.poll_budget_products = poll_budget_products();
     return umma ? launch_ssm_scan_umma(a, (int)p.units, p.blocks, (cudaStream_t)stream) : launch_ssm_scan_mma(a, d->dtype, (int)p.units, p.blocks, (cudaStream_t)stream);
 }

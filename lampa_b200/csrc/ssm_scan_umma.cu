@@ -391,6 +391,14 @@ struct SmC {
     uint64_t in_c, in_b, in_x, in_z, g, y, ds, px, drain;
     uint32_t tslot;
 };
+// Two warps wait in the output pass, and each arms barriers that only the other one waits on: z's (in_z) is armed by the product warp, C's and B's by
+// the copying warp.  Behind C_NEXT their last phases are complete, unless the other one's wait has run out; a barrier must not be armed in an
+// open phase, so whoever arms looks for itself, and gives up as well where it finds one.
+__device__ __forceinline__ void complete_or_dead(uint64_t* bar, int c, bool& dead, int32_t* status) {
+    if (dead || mbar_try_wait(bar, c & 1)) return;
+    dead = true;
+    set_status(status, LAMPA_ERR_TIMEOUT, 54, c & 1);
+}
 
 // z sigmoid(z) of two values.  With t = e^-|z| the denominator 1 + t lies in [1, 2], where its reciprocal is a cubic and one Newton step:
 // 1 - v p(v) = T4(2v - 3) / T4(3) with the Chebyshev polynomial T4, 1 / 577 at most, squared by the step: 3e-6.  (Through the
@@ -449,8 +457,8 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a, con
                        dX0 = umma_desc_mn128(smem_u32(s.x[0])), dX1 = umma_desc_mn128(smem_u32(s.x[1]));
         auto scores_and_states = [&](int c) {     // G of chunk c as soon as its tiles are there, Y when the last chunk's has been read
             if (lane == 0) {
-                mbar_wait(&s.in_c, c & 1, dead, a.status, 54, a.poll_budget);
-                mbar_wait(&s.in_b, c & 1, dead, a.status, 54, a.poll_budget);
+                mbar_wait(&s.in_c, c & 1, dead, a.status, 54, a.poll_budget_products);
+                mbar_wait(&s.in_b, c & 1, dead, a.status, 54, a.poll_budget_products);
                 tc_fence_after();
 #pragma unroll
                 for (int k = 0; k < 4 * NPAN; ++k) {
@@ -489,6 +497,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a, con
                 tma_store_3d(&maps.y, slab, h0, t, s.z[0]);
                 if (hl + 1 < hpg) tma_store_3d(&maps.y, slab, h1, t, s.z[1]);
                 bulk_commit();
+                if (a.z_vec) complete_or_dead(&s.in_z, c - 1, dead, a.status);
                 bulk_wait_read();
                 if (a.z_vec && !dead) load_z(c);
             }
@@ -543,7 +552,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a, con
             tma_load_3d(s.x[0], &maps.x, slab, h0, tok(c), &s.in_x);
             tma_load_3d(s.x[1], &maps.x, slab, h1, tok(c), &s.in_x);
         };
-        // A wait that ran out (`dead`) ends the loading; what was asked for is drained at the end.
+        // A wait that ran out (`dead`), or one of the product warp's whose copy is not there yet, ends the loading; what was asked for is drained at the end.
         int asked_c = 1, asked_b = 1, asked_x = 1;
         if (lane == 0) { load_x(0); load_C(0); load_B(0); }
         __syncwarp();
@@ -559,6 +568,10 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a, con
             tc_fence_before();
             nb_arrive<CC>(C_G);
             if (lane == 0) {
+                if (more) {
+                    complete_or_dead(&s.in_c, c, dead, a.status);
+                    complete_or_dead(&s.in_b, c, dead, a.status);
+                }
                 wait(&s.y, c);
                 if (more && !dead) { load_C(c + 1); ++asked_c; }
             }

@@ -59,3 +59,30 @@ def test_scan_decay_beyond_the_largest_float(lb, form, dtype):  # noqa: F811
     a["A"] = torch.tensor([-1e4, -2.0], device="cuda")
     a["dt"][..., 0] = torch.where(a["dt"][..., 0] < 1, a["dt"][..., 0] * 1e-3, a["dt"][..., 0])
     check_scan(lb, a, softplus=False)
+
+
+# ---- scan: one of two waiting warps gives up -----------------------------------------------------------
+@pytest.mark.parametrize("products,others", [(0, 1 << 16), (1, 1 << 16), (1 << 16, 0), (1 << 16, 1), (0, 1), (1, 0)])
+def test_scan_one_warp_gives_up(lb, products, others):  # noqa: F811
+    """The output pass ends and says so whichever of its two waiting warps runs out (test_state_space_handover.py has the model), and the next call is right"""
+    from lampa_b200 import _lib
+    for H, T, z in ((4, 1000, True), (48, 1500, True), (48, 1500, False)):       # blocks of one chunk, and of several
+        a = scan_inputs(12, 1, T, H, 64, 1, 128, BF, z=z, h0=True)
+        want = lb.state_space_scan(**a, output_final_state=True)
+        try:
+            assert _lib.lib().lampa_debug_set_poll_budget(others) == 0 and _lib.lib().lampa_debug_set_product_poll_budget(products) == 0
+            lb.state_space_scan(**a, output_final_state=True)
+            torch.cuda.synchronize()
+        finally:
+            _lib.lib().lampa_debug_set_poll_budget(1 << 22)
+        if 0 in (products, others):
+            with pytest.raises(lb.LampaError):
+                lb.check_status()
+        else:                                      # a single poll may wait long enough in hardware to succeed
+            try:
+                lb.check_status()
+            except lb.LampaError:
+                pass
+        again = lb.state_space_scan(**a, output_final_state=True)
+        lb.check_status()
+        assert torch.equal(want[0], again[0]) and torch.equal(want[1], again[1])
