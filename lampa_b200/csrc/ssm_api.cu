@@ -36,12 +36,14 @@ struct Plan { int bl, nb; int64_t units; bool blocks; size_t state_bytes, bytes;
 Plan plan_of(const lampa_ssm_desc* d, bool umma) {
     Plan p;
     const int64_t n_tok = (int64_t)d->B * d->T;
+    const int nseq = d->nseq ? d->nseq : d->B;
     p.bl = block_tokens(d, umma);
     p.nb = (int)(((int64_t)d->T + p.bl - 1) / p.bl);
-    p.units = ssm_units(n_tok, d->nseq ? d->nseq : d->B, p.nb, p.bl, d->nseq > 0);
+    p.units = ssm_units(n_tok, nseq, p.nb, p.bl, d->nseq > 0);
     p.blocks = d->T > p.bl;                                        // some sequence may have more than one
-    p.state_bytes = (size_t)p.units * d->H * d->P * d->N * 4;
-    p.bytes = p.blocks || umma ? p.state_bytes + (size_t)p.units * d->H * 4 : 0;
+    const int64_t slots = p.blocks ? ssm_slots(n_tok, nseq, p.nb, p.bl, d->nseq > 0) : 0;
+    p.state_bytes = (size_t)slots * d->H * d->P * d->N * 4;
+    p.bytes = p.state_bytes + (size_t)slots * d->H * 4;
     return p;
 }
 
@@ -90,7 +92,6 @@ extern "C" int lampa_ssm_scan(const lampa_ssm_desc* d, const void* x, int64_t x_
     a.z_vec = z && rows16(z, z_tok, z_head) && steps_on(z_tok, z_head, d->H);
     a.z_pair = z && d->P % 2 == 0 && (((uintptr_t)z | (uintptr_t)(z_tok * 2) | (uintptr_t)(z_head * 2)) & 3) == 0;
     a.y_pair = d->P % 2 == 0 && ((uintptr_t)y & 3) == 0;
-    a.whole = umma;
     a.poll_budget = poll_budget();
     a.poll_budget_products = poll_budget_products();
     return umma ? launch_ssm_scan_umma(a, (int)p.units, p.blocks, (cudaStream_t)stream) : launch_ssm_scan_mma(a, d->dtype, (int)p.units, p.blocks, (cudaStream_t)stream);

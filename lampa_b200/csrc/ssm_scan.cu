@@ -283,15 +283,15 @@ __global__ void __launch_bounds__(THREADS) ssm_state_kernel(SsmArgs a) {
         update_state(st, s, expf(g), 3);
         log_dec += g;
     }
-    float* out = a.blk + ((int64_t)blockIdx.x * a.H + h) * a.P * a.N;
+    float* out = a.blk + (u.slot * a.H + h) * a.P * a.N;
     each_state<NP, PT>(st, [&](int p, int n, float v) {
         if (p0 + p < a.P && n < a.N) out[(int64_t)(p0 + p) * a.N + n] = v;
     });
-    if (threadIdx.x == 0 && blockIdx.z == 0) a.blk_dec[(int64_t)blockIdx.x * a.H + h] = log_dec;
+    if (threadIdx.x == 0 && blockIdx.z == 0) a.blk_dec[u.slot * a.H + h] = log_dec;
 }
 
 // Over the blocks of a sequence: what enters each of them takes the place of what it makes of an empty state.  Also the final state,
-// but for sequences of one block, whose only CTA writes it.  V state elements to a thread, AHEAD blocks asked for before the first is used
+// but for sequences of one block, whose only CTA writes it (in the output pass, or the block kernel of the tcgen05 form).  V state elements to a thread, AHEAD blocks asked for before the first is used
 // (one by one: 27 us instead of 5 for 18 blocks of 16 heads of 64 x 128).
 template <int V, int AHEAD>
 __global__ void __launch_bounds__(256) ssm_pass_kernel(SsmArgs a) {
@@ -303,13 +303,13 @@ __global__ void __launch_bounds__(256) ssm_pass_kernel(SsmArgs a) {
     if (a.cu) {
         bos = a.cu[seq]; eos = a.cu[seq + 1];
         if (bos < 0 || eos < bos || eos > a.n_tok) return;         // reported by the output kernel
-        u0 = ssm_block_of(a, bos) + seq;
+        u0 = ssm_block_of(a, bos, a.bl / 2);
     }
     if (e >= pn) return;
     const int64_t len = eos - bos, out = ((int64_t)seq * a.H + h) * pn + e;
     Vec s = {};
     if (a.h0) s = *reinterpret_cast<const Vec*>(a.h0 + out);
-    if (len > a.bl || (a.whole && a.ht && len > 0)) {
+    if (len > a.bl) {
         const int nb = (int)((len + a.bl - 1) / a.bl);
         float* p = a.blk + (u0 * a.H + h) * pn + e;
         const float* dec = a.blk_dec + u0 * a.H + h;
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(THREADS, NP * PT <= 512 && (DT == LAMPA_BF16 |
     const bool single = u.single(a.bl);
     const int pieces = single && a.ht ? 3 : XP;
     const int64_t pn = (int64_t)a.P * a.N;
-    const float* enter = single ? (a.h0 ? a.h0 + ((int64_t)u.seq * a.H + h) * pn : nullptr) : a.blk + ((int64_t)blockIdx.x * a.H + h) * pn;
+    const float* enter = single ? (a.h0 ? a.h0 + ((int64_t)u.seq * a.H + h) * pn : nullptr) : a.blk + (u.slot * a.H + h) * pn;
     constexpr bool AHEAD = NP <= 64;
     const float Dh = a.D ? a.D[h] : 0.f, A = a.A[h], bias = a.dt_bias ? a.dt_bias[h] : 0.f;
     for (int i = threadIdx.x; i < PT; i += THREADS) s.bad[i] = Q;

@@ -194,6 +194,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_state_umma_kernel(SsmArgs a, c
     SmA& s = *reinterpret_cast<SmA*>(raw);
     SsmUnit u;
     if (!ssm_unit(a, blockIdx.x, u) || u.outside || (u.single(a.bl) && !a.ht)) return;
+    const bool single = PIECES == 3 && u.single(a.bl);             // the whole sequence: from the state that enters it to the final one
     const int hpg = a.H / a.G, pairs = (hpg + 1) / 2, grp = blockIdx.y / pairs, hl = 2 * (blockIdx.y % pairs), slab = blockIdx.z * 64;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h0 = grp * hpg + hl;
     const int chunks = (int)((u.t1 - u.t0 + UQ - 1) / UQ);
@@ -302,7 +303,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_state_umma_kernel(SsmArgs a, c
             p.ask(a, u.t0 + (int64_t)(c + 1) * UQ, rows(c + 1));
             nb_sync<CS>(A_NEXT);
         }
-        if (p.has && lane == 0 && slab == 0) a.blk_dec[(int64_t)blockIdx.x * a.H + h0 + x] = log_dec;
+        if (p.has && lane == 0 && slab == 0 && !single) a.blk_dec[u.slot * a.H + h0 + x] = log_dec;
         nb_sync<ALL>(0);
         return;
     }
@@ -311,9 +312,11 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_state_umma_kernel(SsmArgs a, c
     const Own<NPAN> own(q, half, lane);
     constexpr int PC = Own<NPAN>::PC;
     const bool has = hl + hd < hpg;
+    const int64_t pn = (int64_t)a.P * a.N;
     float st[PC];
+    const float* const enter = single && a.h0 && has && own.n < a.N ? a.h0 + ((int64_t)u.seq * a.H + h0 + hd) * pn + own.n : nullptr;
 #pragma unroll
-    for (int i = 0; i < PC; ++i) st[i] = 0.f;
+    for (int i = 0; i < PC; ++i) st[i] = enter && slab + own.p0 + i < a.P ? enter[(int64_t)(slab + own.p0 + i) * a.N] : 0.f;
     auto take_in = [&](int c) {                   // states <- decay * states + dS of chunk c
         float ds[PC];
         tm_ld<PC>(ds, tm + ((uint32_t)(32 * q) << 16) + 128 * (c & 1) + 64 * hd + own.p0);
@@ -363,7 +366,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_state_umma_kernel(SsmArgs a, c
     nb_sync<CC>(A_END);
     tc_fence_after();
     take_in(chunks - 1);
-    float* const out = a.blk + ((int64_t)blockIdx.x * a.H + h0 + hd) * a.P * a.N;
+    float* const out = single ? a.ht + ((int64_t)u.seq * a.H + h0 + hd) * pn : a.blk + (u.slot * a.H + h0 + hd) * pn;
     if (has && own.n < a.N)
 #pragma unroll
         for (int i = 0; i < PC; ++i)
@@ -655,7 +658,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_umma_kernel(SsmArgs a, con
     {
         const bool single = u.single(a.bl);
         const int64_t pn = (int64_t)a.P * a.N;
-        const float* enter = !has ? nullptr : single ? (a.h0 ? a.h0 + ((int64_t)u.seq * a.H + h) * pn : nullptr) : a.blk + ((int64_t)blockIdx.x * a.H + h) * pn;
+        const float* enter = !has ? nullptr : single ? (a.h0 ? a.h0 + ((int64_t)u.seq * a.H + h) * pn : nullptr) : a.blk + (u.slot * a.H + h) * pn;
         nb_sync<CS>(C_DS);
         const float dec = s.tot[0][hd];
 #pragma unroll
@@ -875,17 +878,19 @@ bool make_map3(CUtensorMap* m, const void* base, int64_t n_tok, int heads, int c
 }
 
 template <int NPAN>
-int launch_pan(const SsmArgs& a, const Maps& maps, int units, bool states, cudaStream_t st) {
+int launch_pan(const SsmArgs& a, const Maps& maps, int units, bool blocks, cudaStream_t st) {
     static std::atomic<uint64_t> ready_s{0}, ready_1{0}, ready_o{0};
     static_assert(sizeof(SmA) <= MAX_SMEM && sizeof(SmC<NPAN>) <= MAX_SMEM, "tiles fit");
     const dim3 grid(units, (unsigned)(a.G * ((a.H / a.G + 1) / 2)), (a.P + 63) / 64);
-    if (states) {
+    if (blocks || a.ht) {
         const auto kernel = a.ht ? ssm_state_umma_kernel<NPAN, 3> : ssm_state_umma_kernel<NPAN, 1>;
         if (!allow_smem(a.ht ? ready_s : ready_1, kernel, (int)sizeof(SmA))) return LAMPA_ERR_CUDA;
         {
             ProfScope prof("ssm_state", st);
             if (launch_chained(kernel, grid, dim3(THREADS), sizeof(SmA), st, a, maps) != cudaSuccess) return LAMPA_ERR_CUDA;
         }
+    }
+    if (blocks || (a.cu && a.ht)) {
         const int rc = launch_ssm_pass(a, st);
         if (rc != LAMPA_OK) return rc;
     }
@@ -903,8 +908,7 @@ int launch_ssm_scan_umma(SsmArgs a, int units, bool blocks, cudaStream_t st) {
     maps.z = maps.x;
     if (!make_map3(&maps.y, a.y, a.n_tok, a.H, a.P, (int64_t)a.H * a.P, a.P)) return LAMPA_ERR_CUDA;
     a.z_vec = a.z_vec && make_map3(&maps.z, a.z, a.n_tok, a.H, a.P, a.z_tok, a.z_head);
-    const bool states = blocks || a.ht;
-    return a.N <= 64 ? launch_pan<1>(a, maps, units, states, st) : launch_pan<2>(a, maps, units, states, st);
+    return a.N <= 64 ? launch_pan<1>(a, maps, units, blocks, st) : launch_pan<2>(a, maps, units, blocks, st);
 }
 
 }  // namespace lampa

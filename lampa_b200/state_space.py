@@ -65,8 +65,8 @@ def state_space_scan(
     have a type of its own.  Any P, N up to 256, any lengths from 0 on; rows
     behind the last entry of cu_seqlens come out as zero.  D None: no skip; z None: no gate.
     A times a step is meant to be at most 0 (a decay); growth is computed too as long as e^(A sum d) over any 128 tokens is finite.
-    The last bits of y and of the states depend on how long the whole call is (the tokens are cut into blocks), those of two
-    equal calls do not differ.
+    The last bits of y and of the states depend on how long the whole call is (the tokens are cut into blocks), those of y also on
+    whether a final state is asked for; those of two equal calls do not differ.
     Offsets on the device that fall or leave the input are reported through `check_status()`.
     """
     r = L.native.ssm_scan(x, dt, A, B, C, D, z, dt_bias, initial_state, cu_seqlens, bool(dt_softplus), bool(output_final_state), True) \

@@ -86,3 +86,47 @@ def test_scan_one_warp_gives_up(lb, products, others):  # noqa: F811
         again = lb.state_space_scan(**a, output_final_state=True)
         lb.check_status()
         assert torch.equal(want[0], again[0]) and torch.equal(want[1], again[1])
+
+
+# ---- scan: what a state is kept for ----------------------------------------------------------------------
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_scan_of_a_batch_whose_sequences_are_one_block_each(lb, form, dtype, given):  # noqa: F811
+    """Several chunks, no workspace: the block kernel of the tcgen05 form goes from the entering state to the final one"""
+    for P, N in ((64, 128), (40, 24)):
+        a = scan_inputs(41 + P, 10, 300, 32, P, 1, N, dtype, z=True, h0=given, decay=0.1)
+        y, _ = check_scan(lb, a)
+        assert torch.equal(y, lb.state_space_scan(**a)[0])
+
+
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_scan_of_a_packed_batch_that_one_sequence_dominates(lb, form, dtype, given):  # noqa: F811
+    lens = [40] * 7 + [0, 4500, 0, 300, 1, 1000, 129, 128]
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    a = scan_inputs(43, 1, cu[-1] + 5, 8, 64, 1, 64, dtype, z=True, h0=given, nseq=len(lens))
+    off = torch.tensor(cu, device="cuda")
+    y, ht = lb.state_space_scan(**a, output_final_state=True, cu_seqlens=off)
+    assert (y[0, cu[-1]:] == 0).all()
+    cut = {k: (v[:, :cu[-1]] if k in ("x", "dt", "B", "C", "z") else v) for k, v in a.items()}
+    check_scan(lb, cut, cu)
+    check_scan(lb, cut, cu, final=False)
+    for s, n in enumerate(lens):
+        if n == 0:
+            assert torch.equal(ht[s], a["initial_state"][s] if given else torch.zeros_like(ht[s]))
+
+
+def test_scan_of_many_prompts_takes_little_scratch(lb):  # noqa: F811
+    """16 384 packed prompts of 40 tokens: what a call allocates beside y is not a state to each of them"""
+    n, H, P, N = 16384, 4, 64, 64
+    a = scan_inputs(44, 1, 40 * n, H, P, 1, N, BF)
+    off = torch.arange(n + 1, device="cuda") * 40
+    lb.state_space_scan(**a, cu_seqlens=off)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    y, _ = lb.state_space_scan(**a, cu_seqlens=off)
+    assert torch.cuda.max_memory_allocated() - before - 2 * y.numel() < 100 << 20        # a state each would be 1 GB
+    lb.check_status()
