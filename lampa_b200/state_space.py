@@ -39,7 +39,7 @@ def _rows(t: Optional[torch.Tensor], aligned: bool = False) -> Optional[torch.Te
     even = even and (t.shape[-1] <= 1 or t.stride(-1) == 1)
     if aligned:
         even = even and not any(v * t.element_size() % 16 for n, v in zip(t.shape[:-1], t.stride()) if n > 1) and t.data_ptr() % 16 == 0
-    return t if even else t.contiguous()
+    return t if even else t.clone(memory_format=torch.contiguous_format)       # (a dense one at an odd place, too)
 
 
 def state_space_scan(

@@ -130,3 +130,17 @@ def test_scan_of_many_prompts_takes_little_scratch(lb):  # noqa: F811
     y, _ = lb.state_space_scan(**a, cu_seqlens=off)
     assert torch.cuda.max_memory_allocated() - before - 2 * y.numel() < 100 << 20        # a state each would be 1 GB
     lb.check_status()
+
+
+# ---- scan: x, B and C that lie at odd places ----------------------------------------------------------
+@pytest.mark.parametrize("what", ["x", "B", "C"])
+def test_scan_of_dense_inputs_at_odd_places(lb, what):  # noqa: F811
+    """Dense, but not on a 16-byte boundary: copied to one, so that the same kernels run"""
+    a = {k: v.contiguous() if isinstance(v, torch.Tensor) else v for k, v in scan_inputs(31, 1, 400, 2, 64, 1, 64, BF).items()}
+    want = lb.state_space_scan(**a, output_final_state=True)
+    buf = torch.zeros(a[what].numel() + 8, dtype=BF, device="cuda")
+    odd = buf[1:1 + a[what].numel()].view(a[what].shape)
+    odd.copy_(a[what])
+    assert odd.is_contiguous() and odd.data_ptr() % 16
+    got = lb.state_space_scan(**dict(a, **{what: odd}), output_final_state=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
