@@ -219,7 +219,7 @@ def short_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     """Depthwise causal convolution over the tokens of x [B,T,D] for sequences that continue: what lies before a sequence's first
     token is what its cache [N,D,W] holds (W last inputs, as ShortConvolution keeps them; None: zeros).  With output_final_state
     the cache, or a new one, becomes the last W inputs of each sequence, in place, and is returned; that of an empty sequence
-    stays.  weight: [D,W] or [D,1,W], W from 2 to 8; bias: [D]; cu_seqlens: [N+1] with B == 1 (rows behind its last entry come out
+    stays.  weight: [D,W] or [D,1,W], W from 2 to 8; bias: [D], of the weight's type or one of its own; cu_seqlens: [N+1] with B == 1 (rows behind its last entry come out
     as zero).  x may be a part of wider rows.  Returns (y [B,T,D] in x's dtype, cache or None)."""
     from .gated_delta import _check_cu_seqlens, _forward_only, _launched
     from .state_space import _conv_params, _rows

@@ -130,7 +130,7 @@ def state_space_step(
 
     xbc: [B, H*P + 2*G*N], a row's x, B and C before the convolution; dt: [B,H]; z: [B,H,P]; conv_cache: [B, channels, W] in
     xbc's dtype (ShortConvolution's cache: the last W inputs); conv_weight: [channels, W] or [channels, 1, W]; conv_bias:
-    [channels] or None; state: [B,H,P,N] fp32.  Returns y [B,H,P] in xbc's dtype (bf16, fp16 or fp32).  The number of groups
+    [channels] or None, of the weight's type or one of its own; state: [B,H,P,N] fp32.  Returns y [B,H,P] in xbc's dtype (bf16, fp16 or fp32).  The number of groups
     follows from the width of xbc.  Rows of xbc, dt and z may be parts of wider rows.
     """
     if activation not in (None, "silu", "swish"):
@@ -180,4 +180,9 @@ def _conv_params(weight: torch.Tensor, bias: Optional[torch.Tensor], channels: i
         raise ValueError(f"the convolution's weight must be [{channels}, {taps}]")
     if bias is not None and tuple(bias.shape) != (channels,):
         raise ValueError(f"the convolution's bias must be [{channels}]")
-    return w.contiguous(), None if bias is None else bias.detach().to(w.dtype).contiguous()
+    if bias is None:
+        return w.contiguous(), None
+    b = bias.detach()
+    if b.dtype != w.dtype:                        # the kernels take one type for both: fp32 holds either
+        w, b = w.float(), b.float()
+    return w.contiguous(), b.contiguous()

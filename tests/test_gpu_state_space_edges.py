@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests.test_gpu_state_space import BF, F32, FP, check_scan, lb, scan_inputs  # noqa: F401  (lb is a fixture)
+from tests.test_gpu_state_space import BF, F32, FP, check_conv, check_scan, check_step, lb, scan_inputs, step_inputs  # noqa: F401  (lb is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -144,3 +144,15 @@ def test_scan_of_dense_inputs_at_odd_places(lb, what):  # noqa: F811
     assert odd.is_contiguous() and odd.data_ptr() % 16
     got = lb.state_space_scan(**dict(a, **{what: odd}), output_final_state=True)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# ---- a convolution's bias of a type of its own ---------------------------------------------------------
+@pytest.mark.parametrize("w_dtype,b_dtype", [(BF, F32), (FP, F32), (BF, FP), (FP, BF), (F32, BF)])
+def test_bias_keeps_its_bits(lb, w_dtype, b_dtype):  # noqa: F811
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    r = lambda *s: torch.randn(*s, generator=gen, device="cuda")  # noqa: E731
+    x, w, b = r(2, 50, 24).to(F32), (0.01 * r(24, 4)).to(w_dtype), (1 + r(24).abs()).to(b_dtype)
+    check_conv(lb, x, w, b, None, r(2, 24, 4), None)
+    a = step_inputs(6, 3, 2, 8, 1, 8, 4, F32, w_dtype=w_dtype)
+    a.update(conv_weight=a["conv_weight"] * 0.01, conv_bias=(1 + r(32).abs()).to(b_dtype))
+    check_step(lb, a)
