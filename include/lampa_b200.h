@@ -419,7 +419,8 @@ int lampa_ssm_workspace_bytes(const lampa_ssm_desc* d, size_t* bytes);
  * x, z [B*T][H][P], B, C [B*T][G][N], dt [B*T][H]: the innermost axis is contiguous, the distances of the others are given in
  * elements (*_tok from one token to the next, *_head / *_grp from one head / group to the next; heads of dt are neighbours), so that
  * parts of a projection's rows are read in place.  y [B*T][H][P] dense.  A, D, dt_bias [H] fp32 (D, dt_bias, z may be NULL).
- * initial_state, final_state [N_seq][H][P][N] fp32 or NULL, N_seq = nseq or B; they may not overlap.  A[h] d_t is meant to be at
+ * initial_state, final_state [N_seq][H][P][N] fp32 or NULL, N_seq = nseq or B; they may not overlap (a sequence of no tokens: its initial
+ * state, or zero, also where T is 0).  A[h] d_t is meant to be at
  * most 0 (a decay); growth is computed too, as long as e^(A d) over any 128 tokens stays a finite float.
  * cu_seqlens: device int64 [nseq+1] rising from 0; rows of y behind its last entry are zero; an entry that falls or leaves the
  * input sets LAMPA_ERR_BOUNDS and leaves that sequence's outputs undefined.  Every state is found and kept in fp32 (relative

@@ -67,7 +67,15 @@ extern "C" int lampa_ssm_scan(const lampa_ssm_desc* d, const void* x, int64_t x_
                               size_t ws_bytes, int32_t* status, void* stream) {
     if (!desc_ok(d) || (cu_seqlens != nullptr) != (d->nseq > 0)) return LAMPA_ERR_ARG;
     if (!built(d)) return LAMPA_ERR_UNSUPPORTED;
-    if (d->B == 0 || d->T == 0) return LAMPA_OK;
+    if (d->B == 0) return LAMPA_OK;
+    if (d->T == 0) {                                               // no tokens: what enters the sequences is what leaves them
+        if (!final_state) return LAMPA_OK;
+        SsmArgs a = {};
+        a.h0 = initial_state; a.ht = final_state; a.cu = cu_seqlens; a.status = status;
+        a.nseq = d->nseq ? d->nseq : d->B;
+        a.bl = SSM_Q; a.H = d->H; a.P = d->P; a.N = d->N;
+        return launch_ssm_pass(a, (cudaStream_t)stream);
+    }
     if (!x || !dt || !A || !B || !C || !y) return LAMPA_ERR_ARG;
     auto rows16 = [](const void* q, int64_t s0, int64_t s1) { return (((uintptr_t)q | (uintptr_t)(s0 * 2) | (uintptr_t)(s1 * 2)) & 15) == 0; };
     const bool vec = d->P % 8 == 0 && d->N % 8 == 0 && rows16(x, x_tok, x_head) && rows16(B, b_tok, b_grp) && rows16(C, c_tok, c_grp);

@@ -301,6 +301,7 @@ __global__ void __launch_bounds__(256) ssm_pass_kernel(SsmArgs a) {
     const int e = ((blockIdx.x - seq * slabs) * 256 + threadIdx.x) * V;
     int64_t bos = (int64_t)seq * a.T, eos = bos + a.T, u0 = (int64_t)seq * a.nb;
     if (a.cu) {
+        if (a.n_tok == 0 && blockIdx.x == 0 && blockIdx.y == 0) check_offsets(a.cu, a.nseq, 0, a.status, 50);      // (there is no output kernel)
         bos = a.cu[seq]; eos = a.cu[seq + 1];
         if (bos < 0 || eos < bos || eos > a.n_tok) return;         // reported by the output kernel
         u0 = ssm_block_of(a, bos, a.bl / 2);

@@ -156,3 +156,27 @@ def test_bias_keeps_its_bits(lb, w_dtype, b_dtype):  # noqa: F811
     a = step_inputs(6, 3, 2, 8, 1, 8, 4, F32, w_dtype=w_dtype)
     a.update(conv_weight=a["conv_weight"] * 0.01, conv_bias=(1 + r(32).abs()).to(b_dtype))
     check_step(lb, a)
+
+
+# ---- the C entry point of a scan over no tokens ----------------------------------------------------------
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("given", [False, True])
+def test_scan_entry_point_of_no_tokens_has_a_final_state(lb, packed, given):  # noqa: F811
+    import ctypes
+    from lampa_b200 import _lib as L
+    h0 = torch.randn(3, 2, 5, 7, device="cuda") if given else None
+    ht = torch.full((3, 2, 5, 7), 9.0, device="cuda")
+    cu = torch.zeros(4, dtype=torch.int64, device="cuda") if packed else None
+    d = L.SsmDesc(B=1 if packed else 3, T=0, H=2, P=5, N=7, G=1, nseq=3 if packed else 0, dtype=0, dt_dtype=0, dt_softplus=1)
+    dev = torch.device("cuda:0")
+    rc = L.lib().lampa_ssm_scan(ctypes.byref(d), None, 0, 0, None, 0, None, None, 0, 0, None, 0, 0, None, None, 0, 0, None,
+                                L.ptr(h0), L.ptr(cu), None, L.ptr(ht), None, 0, L.ptr(L.status_word(dev)), L.stream_ptr(dev))
+    assert rc == 0
+    lb.check_status()
+    assert torch.equal(ht, h0 if given else torch.zeros_like(ht))
+    if packed:                                     # offsets that leave the (empty) input
+        cu[1] = 4
+        L.check(L.lib().lampa_ssm_scan(ctypes.byref(d), None, 0, 0, None, 0, None, None, 0, 0, None, 0, 0, None, None, 0, 0, None,
+                                       L.ptr(h0), L.ptr(cu), None, L.ptr(ht), None, 0, L.ptr(L.status_word(dev)), L.stream_ptr(dev)), "lampa_ssm_scan")
+        with pytest.raises(lb.LampaError):
+            lb.check_status()
