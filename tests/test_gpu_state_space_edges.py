@@ -180,3 +180,47 @@ def test_scan_entry_point_of_no_tokens_has_a_final_state(lb, packed, given):  # 
                                        L.ptr(h0), L.ptr(cu), None, L.ptr(ht), None, 0, L.ptr(L.status_word(dev)), L.stream_ptr(dev)), "lampa_ssm_scan")
         with pytest.raises(lb.LampaError):
             lb.check_status()
+
+
+# ---- scan: values that are not finite ---------------------------------------------------------------------
+@pytest.mark.parametrize("H", [2, 256])           # blocks of one chunk, and of all of a sequence's
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_scan_spreads_nothing_that_is_not_finite(lb, form, dtype, H):  # noqa: F811
+    """NaN and infinity spoil their sequence from their token on, an x only its column and a dt only its head, in both forms and types"""
+    cu = [0, 70, 370, 410, 540]
+    off = torch.tensor(cu, device="cuda")
+    a = scan_inputs(51, 1, 540, H, 64, 1, 64, dtype, z=True, h0=True, nseq=4)
+    clean, hc = lb.state_space_scan(**a, output_final_state=True, cu_seqlens=off)
+    assert torch.isfinite(clean).all() and torch.isfinite(hc).all()
+    keep = [i for i in range(64) if i != 9]
+    for what, t in (("x", 100), ("x", 134), ("x", 369), ("dt", 200), ("dt", 71), ("B", 70), ("B", 260), ("C", 150), ("initial_state", 70)):
+        for bad in (float("nan"), float("inf"), -float("inf")):
+            if what == "dt" and bad < 0:
+                continue                           # a step of zero
+            b = dict(a, **{what: a[what].clone()})
+            if what == "dt":
+                b["dt"][0, t, 1] = bad
+            elif what == "initial_state":
+                b[what][1, 0, 9, 5] = bad
+            else:
+                b[what][0, t, 0, 9] = bad
+            y, ht = lb.state_space_scan(**b, output_final_state=True, cu_seqlens=off)
+            lb.check_status()
+            where = f"{what} {bad} at {t}"
+            for s in (0, 2, 3):
+                assert torch.equal(y[0, cu[s]:cu[s + 1]], clean[0, cu[s]:cu[s + 1]]) and torch.equal(ht[s], hc[s]), where
+            assert torch.equal(y[0, 70:t], clean[0, 70:t]), where
+            if what in ("x", "initial_state"):
+                # (a state's infinity may meet a decay that has become zero, and then is NaN as 0 * inf is in the recurrence)
+                assert not torch.isfinite(y[0, t:370, 0, 9]).any() and torch.equal(y[0, 70:370, 0][:, keep], clean[0, 70:370, 0][:, keep]), where
+                assert torch.equal(y[0, 70:370, 1:], clean[0, 70:370, 1:]) and torch.equal(ht[1, 0, keep], hc[1, 0, keep]) and torch.equal(ht[1, 1:], hc[1, 1:]), where
+                assert not torch.isfinite(ht[1, 0, 9] if what == "x" else ht[1, 0, 9, 5]).any(), where
+            elif what == "dt":
+                assert not torch.isfinite(y[0, t:370, 1]).any() and not torch.isfinite(ht[1, 1]).any(), where
+                others = [h for h in range(H) if h != 1]
+                assert torch.equal(y[0, 70:370][:, others], clean[0, 70:370][:, others]) and torch.equal(ht[1, others], hc[1, others]), where
+            elif what == "B":
+                assert not torch.isfinite(y[0, t:370]).any() and not torch.isfinite(ht[1, :, :, 9]).any(), where
+                assert torch.equal(ht[1][..., keep], hc[1][..., keep]), where
+            else:
+                assert not torch.isfinite(y[0, t]).any() and torch.equal(y[0, t + 1:370], clean[0, t + 1:370]) and torch.equal(ht, hc), where
