@@ -421,7 +421,8 @@ int lampa_ssm_workspace_bytes(const lampa_ssm_desc* d, size_t* bytes);
  * parts of a projection's rows are read in place.  y [B*T][H][P] dense.  A, D, dt_bias [H] fp32 (D, dt_bias, z may be NULL).
  * initial_state, final_state [N_seq][H][P][N] fp32 or NULL, N_seq = nseq or B; they may not overlap (a sequence of no tokens: its initial
  * state, or zero, also where T is 0).  A[h] d_t is meant to be at
- * most 0 (a decay); growth is computed too, as long as e^(A d) over any 128 tokens stays a finite float.
+ * most 0 (a decay); growth is computed too, as long as e^(A d) over any 128 tokens stays a finite float.  A large d resets the state, and what follows is as exact as
+ * ever; d (C . B) is a float on the way, so that y is not finite where that overflows, even for an x of zero (a d of 1e30 is safe).
  * cu_seqlens: device int64 [nseq+1] rising from 0; rows of y behind its last entry are zero; an entry that falls or leaves the
  * input sets LAMPA_ERR_BOUNDS and leaves that sequence's outputs undefined.  Every state is found and kept in fp32 (relative
  * error below 1e-6); y has one rounding to the input type on the way and its own.  An x, dt, B, C that is not finite spoils its

@@ -47,7 +47,7 @@ __device__ __forceinline__ void to_float(const typename RawRow<DT, VEC>::T& raw,
     else unpack4(raw, v, DT);
 }
 
-// 61 440 x 1 280 in bf16 (315 MB): 64 us, 75 % of the measured bandwidth (SiLU alone takes the special function unit 36).  Eight channels to a
+// 61 440 x 1 280 in bf16 (315 MB): 69 us, 69 % of the measured bandwidth (SiLU alone takes the special function unit 36).  Eight channels to a
 // thread: 129 us, one weight to a load: 211.
 template <int DT, int VEC, int MW, bool EXACT>    // MW: compile-time bound on the number of taps; EXACT: it is their number, four, and weights are 16-bit
 __global__ void __launch_bounds__(128) conv_resume_kernel(ConvArgsR a) {

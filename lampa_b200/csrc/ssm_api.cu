@@ -16,13 +16,13 @@ bool built(const lampa_ssm_desc* d) {
 }
 
 // The tcgen05 kernels take bf16 rows in pieces of 16 bytes, and their state is one operand tile.  A single chunk is one launch of the mma.sync
-// form that ends with the state (64 tokens, 8 heads of 64 x 64: 11.0 us, tcgen05 in three launches 17; 256 such prompts: 89 and 150; 128 tokens:
-// 18.2 and 16.6).
+// form that ends with the state (64 tokens, 8 heads of 64 x 64: 10.6 us, tcgen05 in two launches 16; 256 such prompts: 80 and 108; 128 tokens:
+// 19.6 and 14.9).
 bool umma_shape(const lampa_ssm_desc* d) { return d->dtype == LAMPA_BF16 && d->P % 8 == 0 && d->N % 8 == 0 && d->N <= 128 && d->T > SSM_Q; }
 
 // Tokens per block: enough blocks for eight CTAs to an SM in the mma.sync form (24 001 packed tokens in fp16, 6 heads of 32 x 16: with eight 68 us,
 // six 80, four 71, two 98, when these were compared), for one CTA (of two heads) to an SM in the tcgen05 form, where a second round of CTAs costs as much as the first.
-// Sequences of one length are cut into equally many blocks (four of 2 049 tokens, 8 pairs of heads: 49 us; by all tokens, 160 CTAs, 60); of a packed batch's, each may end in one that is not whole.
+// Sequences of one length are cut into equally many blocks (four of 2 049 tokens, 8 pairs of heads: 49 us, when these were compared; by all tokens, 160 CTAs, 60); of a packed batch's, each may end in one that is not whole.
 int block_tokens(const lampa_ssm_desc* d, bool umma) {
     const int q = umma ? 128 : SSM_Q;
     const int64_t slabs = (d->P + 63) / 64, per = umma ? (int64_t)d->G * ((d->H / d->G + 1) / 2) * slabs : d->H * slabs;

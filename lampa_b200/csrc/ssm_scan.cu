@@ -13,10 +13,11 @@
 // A token whose x is not finite must not reach the rows in front of it through a zero of the mask (0 * NaN): such elements are taken
 // out of the tile, and from their row on the column is NaN, as the recurrence has it.
 //
-// What bounds it: instructions (24 001 packed tokens in fp16, 6 heads of 32 x 16, 60 us in all: output 34 us, issue slots 44 %, tensor pipe 10 %,
-// DRAM 5 %; states 17, pass 9), most of them spent on splitting fp16 into pieces, on decays and on the gate, in four warps a CTA whose phases
-// follow one another.  With tiles and steps loaded just before their use 107 us, with the weighted pieces made from the tile in shared memory 68.  61 440 bf16 tokens, 16 heads of 64 x 128, take 1 120 us here and
-// 214 in the tcgen05 form.
+// What bounds it: instructions (24 001 packed tokens in fp16, 6 heads of 32 x 16, 58 us in all; between events output 35 us, issue slots 45 %, tensor
+// pipe 12 %, DRAM 0.7 TB/s; states 21, pass 15), most of them spent on splitting fp16 into pieces and on the gate, in four warps a CTA whose phases
+// follow one another.  With an exponential for every pair of tokens 61 us, with tiles and steps loaded just before their use 107, with the weighted
+// pieces made from the tile in shared memory 68.  61 440 bf16 tokens, 16 heads of 64 x 128, take 895 us here and 215 in the tcgen05 form (one call after
+// another on the same inputs).
 #include "profile.cuh"
 #include "ssm.cuh"
 

@@ -169,8 +169,8 @@ struct Maps { CUtensorMap x, B, C, z, y; };
 
 // -------------------------------------------------------------------------------------------------
 // What bounds it: shared memory, of which a chunk's 24 products read 192 KB and everything else moves as much again (3.1 k of the 4.1 k cycles
-// of a chunk), and how the products' issue and the element work wait for one another: 61 440 tokens, 16 heads of 64 x 128: 64 us, tensor pipe 35 %,
-// issue slots 41 %, DRAM 34 % (2.2 TB/s).  One step warp for both heads: 75 us; the same warp polling and issuing: 98.
+// of a chunk), and how the products' issue and the element work wait for one another: 61 440 tokens, 16 heads of 64 x 128: 64 us (67 between events), tensor pipe
+// 35 %, issue slots 43 %, DRAM 34 % (2.2 TB/s).  One step warp for both heads: 75 us; the same warp polling and issuing: 98.
 // What a block makes of an empty state.  Its products take d x e^{..} in three bf16 pieces where somebody will see the state (24 bits), in one
 // where only y will.  Every chunk's sum starts from zero and is added to the states in fp32 arithmetic.
 // -------------------------------------------------------------------------------------------------
@@ -379,7 +379,9 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_state_umma_kernel(SsmArgs a, c
 // The output, walking through a block from the state that enters it.
 // What bounds it: a chain of dependent phases of four warps to a scheduler, 10.2 k cycles a chunk of two heads for 3.4 k issue slots (wx 0.9 k,
 // scores 2 - 3 k, states and the entering states' share 1.5 k, gates 2 k beside the products P x, output 0.7 k, hand-overs), and behind that shared
-// memory (4.6 k cycles): 61 440 tokens, 16 heads of 64 x 128: 146 us, issue slots 39 %, tensor pipe 19 %, DRAM 38 % (2.5 TB/s).
+// memory (4.6 k cycles): 61 440 tokens, 16 heads of 64 x 128: 158 us between events, issue slots 39 %, tensor pipe 18 %,
+// DRAM 37 % (2.4 TB/s).  (154 where an exponent between tokens is a difference of sums from the chunk's start, which is wrong behind a large step, and
+// nobody looks at a barrier before arming it.)
 // On the way: tiles by cp.async of the element warps 398 us (spills reach L2 here: shared memory leaves L1 nothing), TMA 198, states in tensor
 // memory instead of registers 159, gates while P x runs 146.  All scores of a row loaded at once: 176 (spills).
 // -------------------------------------------------------------------------------------------------

@@ -65,6 +65,7 @@ def state_space_scan(
     have a type of its own.  Any P, N up to 256, any lengths from 0 on; rows
     behind the last entry of cu_seqlens come out as zero.  D None: no skip; z None: no gate.
     A times a step is meant to be at most 0 (a decay); growth is computed too as long as e^(A sum d) over any 128 tokens is finite.
+    A large step resets the state (d C.B has to stay a finite float, whatever x is: 1e30 is safe).
     The last bits of y and of the states depend on how long the whole call is (the tokens are cut into blocks), those of y also on
     whether a final state is asked for; those of two equal calls do not differ.
     Offsets on the device that fall or leave the input are reported through `check_status()`.
